@@ -228,6 +228,93 @@ TK_API int tk_peer_release(void* ptr);
 TK_API int tk_copy_rows(void* dst, int64_t dst_ld, const void* src, int64_t src_ld, int64_t row_bytes, int64_t rows,
                         void* stream);
 
+/* A paged key-value cache. No counterpart in the reference, whose forward
+ * recomputes every key and value; this is what generating token after token
+ * with the stack needs. The pool is fp16 [layers, num_pages, 2 (k, v), Hkv,
+ * page_size, hd], each page contiguous; the books are int32 on the device and
+ * all owned by the caller:
+ *   page_table [max_seqs, table_width] page of tokens [k * page_size, ...)
+ *   seq_lens   [max_seqs]              tokens cached, 0 for an empty slot
+ *   ref_counts [num_pages]             sequences that hold the page
+ *   free_mask  [words]                 bit p % 32 of word p / 32: page p free;
+ *                                      words = ceil(num_pages / 32) rounded up
+ *                                      to a multiple of 4, 16-byte aligned
+ *   status     [1]                     0, or why a call was refused (tk_cache_status)
+ *   live       [1]                     pages in use after tk_cache_compact
+ *   scratch    [3 * num_pages + 1]     contents never matter between calls
+ * page_size is a power of two in 16..256; max_seqs <= 8192, table_width and
+ * num_pages <= 2^20. Pages are taken lowest first in the order of the call's
+ * entries, so the state that a call leaves depends on its arguments and the
+ * books alone. A call on a cache applies whole or not at all: when an entry
+ * is refused nothing changes, the status word and the device error word are
+ * set, and until the caller zeroes the status word later calls on the cache
+ * do nothing. Slot lists are int32 on the device, at most 8192 entries, each
+ * slot at most once; slot -1 is padding. Calls on one cache must be ordered
+ * on the GPU. */
+typedef struct tk_cache {
+  int32_t* page_table;
+  int32_t* seq_lens;
+  int32_t* ref_counts;
+  uint32_t* free_mask;
+  int32_t* status;
+  int32_t* live;
+  int32_t* scratch;
+  void* pool;
+  int64_t max_seqs, table_width, num_pages, page_size, layers, kv_heads, hd;
+} tk_cache;
+
+typedef enum tk_cache_status {
+  TK_CACHE_OUT_OF_PAGES = 1,  /* fewer free pages than the call needs             */
+  TK_CACHE_BAD_SLOT = 2,      /* slot out of range or twice, or a negative count  */
+  TK_CACHE_TOO_LONG = 4,      /* longer than the slot's row of the page table     */
+  TK_CACHE_BAD_PAGE = 8,      /* the page table names a page outside the pool     */
+  TK_CACHE_NOT_EMPTY = 16     /* a slot that has to be empty is not               */
+} tk_cache_status;
+
+/* Sequence slots[i] grows by counts[i] tokens and takes the pages that they
+ * reach into; require_empty refuses slots that hold tokens already. */
+TK_API int tk_cache_reserve(const tk_cache* cache, const int32_t* slots, const int32_t* counts, int64_t n,
+                            int require_empty, void* stream);
+/* Empty slot dst[i] becomes a copy of sequence src[i]: full pages are shared,
+ * the used rows of a partial last page are copied into a page of its own. */
+TK_API int tk_cache_fork(const tk_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+/* Slots become empty; pages that nothing else holds become free. */
+TK_API int tk_cache_release(const tk_cache* cache, const int32_t* slots, int64_t n, void* stream);
+/* The n live pages move to ids 0..n-1: the k-th live page at or above n into
+ * the k-th free page below it, in every layer. n goes to `live`. */
+TK_API int tk_cache_compact(const tk_cache* cache, void* stream);
+/* Data of whole pages src[i] -> dst[i] in every layer; the books stay as they
+ * are. No dst page may be named twice or be among the src pages. */
+TK_API int tk_cache_copy_pages(const tk_cache* cache, const int32_t* src, const int32_t* dst, int64_t n,
+                               void* stream);
+/* Sets free_mask from ref_counts (after the caller filled the books). */
+TK_API int tk_cache_rebuild(const tk_cache* cache, void* stream);
+/* Keys and values of the last counts[b] tokens of sequence slots[b] (after
+ * tk_cache_reserve): k, v fp16, logically [B, Hkv, S, hd] with shared strides
+ * (elements, multiples of 8) and a contiguous last dimension; token t <
+ * counts[b] of row b goes to position seq_len - counts[b] + t. counts NULL: S
+ * tokens a row. */
+TK_API int tk_cache_store(const tk_cache* cache, int64_t layer, const void* k, const void* v, int64_t stride_b,
+                          int64_t stride_h, int64_t stride_s, const int32_t* slots, const int32_t* counts, int64_t B,
+                          int64_t S, void* stream);
+
+/* Attention of one new token per row over a layer of the cache. The token is
+ * the last of its sequence (seq_len counts it); it sees key j when
+ * seq_len - 1 - j < window or j < sinks (window 0: every key).
+ *   q            : fp16 [B, H, hd], strides in elements, H % Hkv == 0
+ *   k_new, v_new : optional fp16 [B, Hkv, hd] with shared strides: the new
+ *                  token's key and value, written into its page and used
+ *                  (absent: they are in the cache already)
+ *   slots        : int32 [B] (each sequence once when k_new is given); NULL:
+ *                  row b is sequence b. Rows with slot -1 are left untouched
+ *   out          : fp16 [B, H*hd], row stride ld_out
+ * An empty sequence gives zeros. Positions past seq_len and hidden keys may
+ * hold anything. hd in {8, 16, 32, 64, 128, 256}; scale > 0. */
+TK_API int tk_attn_decode(const tk_cache* cache, int64_t layer, const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                          const void* k_new, const void* v_new, int64_t new_stride_b, int64_t new_stride_h,
+                          const int32_t* slots, void* out, int64_t ld_out, int64_t B, int64_t H, float scale,
+                          int64_t window, int64_t sinks, void* stream);
+
 /* Guard probes, same meaning as the reference's can_fuse
  * (src/fused_kernels.py:62-64) and attention_supported
  * (src/kernels.py:96-103): 1 when the kernels accept the shape. */

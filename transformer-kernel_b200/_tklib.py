@@ -33,6 +33,18 @@ STATUS_NAMES = {
 
 # name -> (restype, argtypes); mirrors include/tk_b200.h
 _P, _I, _I64, _F, _U64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_uint64
+
+
+class Cache(ctypes.Structure):
+    """tk_cache: a paged key-value cache's device pointers and sizes."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("page_table", "seq_lens", "ref_counts", "free_mask", "status",
+                                                     "live", "scratch", "pool")]
+    _fields_ += [(name, ctypes.c_int64) for name in ("max_seqs", "table_width", "num_pages", "page_size", "layers",
+                                                     "kv_heads", "hd")]
+
+
+_C = ctypes.POINTER(Cache)
 SIGNATURES = {
     "tk_layernorm": (_I, [_P, _I, _I64, _P, _I, _I64, _P, _I64, _P, _P, _F, _P, _I, _I64, _P, _I64, _I64, _I64,
                           _P]),
@@ -56,6 +68,15 @@ SIGNATURES = {
     "tk_gemm_tiles_set": (_I, [_I64, _I64, _I64, _I, _I]),
     "tk_gemm_tiles_clear": (_I, []),
     "tk_gemm_tiles_chosen": (_I, [_I64, _I64, _I64, _I]),
+    "tk_cache_reserve": (_I, [_C, _P, _P, _I64, _I, _P]),
+    "tk_cache_fork": (_I, [_C, _P, _P, _I64, _P]),
+    "tk_cache_release": (_I, [_C, _P, _I64, _P]),
+    "tk_cache_compact": (_I, [_C, _P]),
+    "tk_cache_copy_pages": (_I, [_C, _P, _P, _I64, _P]),
+    "tk_cache_rebuild": (_I, [_C, _P]),
+    "tk_cache_store": (_I, [_C, _I64, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _P]),
+    "tk_attn_decode": (_I, [_C, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _F, _I64, _I64,
+                            _P]),
     "tk_peer_export": (_I, [_P, _P, ctypes.POINTER(ctypes.c_int64)]),
     "tk_peer_import": (_I, [_P, _I64, ctypes.POINTER(ctypes.c_void_p)]),
     "tk_peer_release": (_I, [_P]),

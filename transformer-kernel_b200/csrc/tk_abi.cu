@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
@@ -15,9 +16,11 @@
 #include <vector>
 
 #include "tk_attn.cuh"
+#include "tk_attn_decode.cuh"
 #include "tk_attn_wide.cuh"
 #include "tk_gemm.cuh"
 #include "tk_layernorm.cuh"
+#include "tk_paged.cuh"
 #include "tk_stack_small.cuh"
 #include "tk_ptx.cuh"
 #include "../../include/tk_b200.h"
@@ -113,6 +116,7 @@ struct DeviceInfo {
   bool gemm_attr_set[4][5] = {};
   bool attn_attr_set[5] = {};
   bool small_attr_set[2] = {};
+  bool decode_attr_set[5][2] = {};
 };
 std::mutex g_dev_mu;
 DeviceInfo g_dev[64];
@@ -839,6 +843,329 @@ int tk_attn_fwd(const void* q, const void* k, const void* v, int64_t stride_b, i
 
 // ----------------------------------------------------------------------------
 // peer memory (CUDA IPC) and row copies
+// ----------------------------------------------------------------------------
+// paged key-value cache
+// ----------------------------------------------------------------------------
+}  // extern "C"
+
+namespace {
+
+int check_cache(const char* fn, const tk_cache* c, tk::paged::Books* b, tk::paged::Pool* pool) {
+  if (c == nullptr) return fail(TK_ERR_INVALID, "%s: null cache", fn);
+  if (c->page_table == nullptr || c->seq_lens == nullptr || c->ref_counts == nullptr || c->free_mask == nullptr ||
+      c->status == nullptr || c->live == nullptr || c->scratch == nullptr || c->pool == nullptr)
+    return fail(TK_ERR_INVALID, "%s: null pointer in the cache", fn);
+  if (c->max_seqs < 1 || c->max_seqs > tk::paged::kMaxEntries || c->table_width < 1 || c->table_width > (1 << 20) ||
+      c->num_pages < 1 || c->num_pages > (1 << 20) || c->layers < 1 || c->layers > (1 << 16) || c->kv_heads < 1 ||
+      c->kv_heads > (1 << 16))
+    return fail(TK_ERR_INVALID, "%s: cache sizes out of range (max_seqs <= 8192, table_width and num_pages <= 2^20)",
+                fn);
+  if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
+    return fail(TK_ERR_UNSUPPORTED, "%s: page_size %lld is not a power of two in 16..256", fn,
+                (long long)c->page_size);
+  if (!tk_attn_supported(c->hd))
+    return fail(TK_ERR_UNSUPPORTED, "%s: head_dim %lld not in {8,16,32,64,128,256}", fn, (long long)c->hd);
+  if (!aligned(c->pool, 16) || !aligned(c->free_mask, 16))
+    return fail(TK_ERR_INVALID, "%s: pool and free_mask need 16-byte alignment", fn);
+  b->table = c->page_table;
+  b->lens = c->seq_lens;
+  b->refs = c->ref_counts;
+  b->free_mask = c->free_mask;
+  b->status = c->status;
+  b->live = c->live;
+  b->scratch = c->scratch;
+  b->width = c->table_width;
+  b->max_seqs = static_cast<int>(c->max_seqs);
+  b->num_pages = static_cast<int>(c->num_pages);
+  b->mask_words = static_cast<int>((c->num_pages + 127) / 128 * 4);
+  b->page_shift = 0;
+  while ((1 << b->page_shift) < c->page_size) ++b->page_shift;
+  pool->base = static_cast<uint4*>(c->pool);
+  pool->row_vecs = static_cast<int>(c->hd / 8);
+  pool->page_vecs = 2 * c->kv_heads * c->page_size * pool->row_vecs;
+  pool->layer_vecs = c->num_pages * pool->page_vecs;
+  pool->layers = static_cast<int>(c->layers);
+  return TK_OK;
+}
+
+int check_list(const char* fn, const int32_t* a, const int32_t* b, int64_t n) {
+  if (n < 0 || n > tk::paged::kMaxEntries)
+    return fail(TK_ERR_INVALID, "%s: %lld entries (at most %d a call)", fn, (long long)n, tk::paged::kMaxEntries);
+  if (n > 0 && (a == nullptr || b == nullptr)) return fail(TK_ERR_INVALID, "%s: null list", fn);
+  return TK_OK;
+}
+
+size_t plan_smem(int64_t n, const tk::paged::Books& b) {
+  return static_cast<size_t>(n) * 4 + static_cast<size_t>((b.max_seqs + 31) / 32) * 4;
+}
+
+int launched(cudaError_t e, const char* fn) {
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? TK_OK : cuda_fail(e, fn);
+}
+
+// The decode kernels: head_dim index and whether a tile holds more than eight query heads.
+template <int HD, bool TWO>
+int launch_decode(DeviceInfo* info, int slot, const CUtensorMap& mk, const CUtensorMap& mv,
+                  const tk::decode::Params& p, cudaStream_t s) {
+  auto kern = tk::decode::decode_kernel<HD, TWO>;
+  {
+    std::lock_guard<std::mutex> lk(g_dev_mu);
+    if (!info->decode_attr_set[slot][TWO]) {
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           tk::decode::Cfg<HD>::SMEM_BYTES);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(decode smem)");
+      info->decode_attr_set[slot][TWO] = true;
+    }
+  }
+  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(p.B) * p.Hkv * p.gtiles);
+  return launched(launch(kern, dim3(grid), dim3(tk::decode::kThreads), tk::decode::Cfg<HD>::SMEM_BYTES, s, true, mk,
+                         mv, p),
+                  "tk_attn_decode launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+int tk_cache_reserve(const tk_cache* cache, const int32_t* slots, const int32_t* counts, int64_t n, int require_empty,
+                     void* stream) {
+  g_last_error.clear();
+  tk::paged::Books b;
+  tk::paged::Pool pool;
+  if (int st = check_cache("tk_cache_reserve", cache, &b, &pool)) return st;
+  if (int st = check_list("tk_cache_reserve", slots, counts, n)) return st;
+  if (n == 0) return TK_OK;
+  int dev;
+  DeviceInfo* info;
+  if (int st = current_device(&dev, &info)) return st;
+  return launched(launch(tk::paged::reserve_kernel, dim3(1), dim3(tk::paged::kPlanThreads), plan_smem(n, b),
+                         static_cast<cudaStream_t>(stream), true, b, slots, counts, static_cast<int>(n),
+                         require_empty ? 1 : 0),
+                  "tk_cache_reserve launch");
+}
+
+int tk_cache_fork(const tk_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream) {
+  g_last_error.clear();
+  tk::paged::Books b;
+  tk::paged::Pool pool;
+  if (int st = check_cache("tk_cache_fork", cache, &b, &pool)) return st;
+  if (int st = check_list("tk_cache_fork", src, dst, n)) return st;
+  if (n == 0) return TK_OK;
+  int dev;
+  DeviceInfo* info;
+  if (int st = current_device(&dev, &info)) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (int st = launched(launch(tk::paged::fork_plan_kernel, dim3(1), dim3(tk::paged::kPlanThreads), plan_smem(n, b), s,
+                               true, b, src, dst, static_cast<int>(n)),
+                        "tk_cache_fork launch"))
+    return st;
+  // a pair copies at most one page per layer: enough CTAs that each thread moves a few vectors
+  const int64_t vecs = pool.layers * pool.page_vecs;
+  const int64_t chunks = std::min<int64_t>((vecs + 1023) / 1024, std::max<int64_t>(1, 8 * info->sms / n));
+  return launched(launch(tk::paged::fork_apply_kernel, dim3(static_cast<unsigned>(n), static_cast<unsigned>(chunks)),
+                         dim3(256), 0, s, true, b, pool, src, dst),
+                  "tk_cache_fork launch");
+}
+
+int tk_cache_release(const tk_cache* cache, const int32_t* slots, int64_t n, void* stream) {
+  g_last_error.clear();
+  tk::paged::Books b;
+  tk::paged::Pool pool;
+  if (int st = check_cache("tk_cache_release", cache, &b, &pool)) return st;
+  if (int st = check_list("tk_cache_release", slots, slots, n)) return st;
+  if (n == 0) return TK_OK;
+  int dev;
+  DeviceInfo* info;
+  if (int st = current_device(&dev, &info)) return st;
+  return launched(launch(tk::paged::release_kernel, dim3(static_cast<unsigned>(n)), dim3(256), plan_smem(0, b),
+                         static_cast<cudaStream_t>(stream), true, b, slots, static_cast<int>(n)),
+                  "tk_cache_release launch");
+}
+
+int tk_cache_compact(const tk_cache* cache, void* stream) {
+  g_last_error.clear();
+  tk::paged::Books b;
+  tk::paged::Pool pool;
+  if (int st = check_cache("tk_cache_compact", cache, &b, &pool)) return st;
+  int dev;
+  DeviceInfo* info;
+  if (int st = current_device(&dev, &info)) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int* moved = b.scratch + 3 * static_cast<int64_t>(b.num_pages);
+  if (int st = launched(launch(tk::paged::compact_plan_kernel, dim3(1), dim3(tk::paged::kPlanThreads), 0, s, true, b,
+                               moved),
+                        "tk_cache_compact launch"))
+    return st;
+  return launched(launch(tk::paged::compact_apply_kernel, dim3(8u * info->sms), dim3(256), 0, s, true, b, pool,
+                         static_cast<const int*>(moved)),
+                  "tk_cache_compact launch");
+}
+
+int tk_cache_copy_pages(const tk_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream) {
+  g_last_error.clear();
+  tk::paged::Books b;
+  tk::paged::Pool pool;
+  if (int st = check_cache("tk_cache_copy_pages", cache, &b, &pool)) return st;
+  if (int st = check_list("tk_cache_copy_pages", src, dst, n)) return st;
+  if (n == 0) return TK_OK;
+  int dev;
+  DeviceInfo* info;
+  if (int st = current_device(&dev, &info)) return st;
+  const int64_t vecs = pool.layers * pool.page_vecs;
+  const int64_t chunks = std::min<int64_t>((vecs + 1023) / 1024, std::max<int64_t>(1, 8 * info->sms / n));
+  return launched(launch(tk::paged::copy_pages_kernel, dim3(static_cast<unsigned>(n), static_cast<unsigned>(chunks)),
+                         dim3(256), 0, static_cast<cudaStream_t>(stream), true, pool, src, dst, b.num_pages),
+                  "tk_cache_copy_pages launch");
+}
+
+int tk_cache_rebuild(const tk_cache* cache, void* stream) {
+  g_last_error.clear();
+  tk::paged::Books b;
+  tk::paged::Pool pool;
+  if (int st = check_cache("tk_cache_rebuild", cache, &b, &pool)) return st;
+  int dev;
+  DeviceInfo* info;
+  if (int st = current_device(&dev, &info)) return st;
+  return launched(launch(tk::paged::free_mask_kernel, dim3(static_cast<unsigned>((b.mask_words + 255) / 256)),
+                         dim3(256), 0, static_cast<cudaStream_t>(stream), true, b),
+                  "tk_cache_rebuild launch");
+}
+
+int tk_cache_store(const tk_cache* cache, int64_t layer, const void* k, const void* v, int64_t stride_b,
+                   int64_t stride_h, int64_t stride_s, const int32_t* slots, const int32_t* counts, int64_t B,
+                   int64_t S, void* stream) {
+  g_last_error.clear();
+  tk::paged::Books b;
+  tk::paged::Pool pool;
+  if (int st = check_cache("tk_cache_store", cache, &b, &pool)) return st;
+  if (int st = check_list("tk_cache_store", slots, slots, B)) return st;
+  if (layer < 0 || layer >= pool.layers)
+    return fail(TK_ERR_INVALID, "tk_cache_store: layer %lld of %d", (long long)layer, pool.layers);
+  if (S < 0 || S > (1ll << 31) - 1) return fail(TK_ERR_INVALID, "tk_cache_store: S = %lld", (long long)S);
+  if (B == 0 || S == 0) return TK_OK;
+  if (k == nullptr || v == nullptr) return fail(TK_ERR_INVALID, "tk_cache_store: null pointer");
+  if (stride_b % 8 || stride_h % 8 || stride_s % 8 || stride_b < 0 || stride_h < 0 || stride_s < 0 ||
+      !aligned(k, 16) || !aligned(v, 16))
+    return fail(TK_ERR_INVALID, "tk_cache_store: k/v need 16-byte aligned bases and strides (multiples of 8)");
+  int dev;
+  DeviceInfo* info;
+  if (int st = current_device(&dev, &info)) return st;
+  tk::paged::StoreParams p;
+  p.k = static_cast<const __half*>(k);
+  p.v = static_cast<const __half*>(v);
+  p.stride_b = stride_b;
+  p.stride_h = stride_h;
+  p.stride_s = stride_s;
+  p.slots = slots;
+  p.counts = counts;
+  p.pages = pool.base + layer * pool.layer_vecs;
+  p.page_vecs = pool.page_vecs;
+  p.S = static_cast<int>(S);
+  p.heads = static_cast<int>(cache->kv_heads);
+  p.row_vecs = pool.row_vecs;
+  const int64_t vecs = S * p.heads * p.row_vecs;
+  const int64_t blocks = std::min<int64_t>((vecs + 255) / 256, std::max<int64_t>(1, 16ll * info->sms / B));
+  return launched(launch(tk::paged::store_kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(B)),
+                         dim3(256), 0, static_cast<cudaStream_t>(stream), true, b, p),
+                  "tk_cache_store launch");
+}
+
+int tk_attn_decode(const tk_cache* cache, int64_t layer, const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                   const void* k_new, const void* v_new, int64_t new_stride_b, int64_t new_stride_h,
+                   const int32_t* slots, void* out, int64_t ld_out, int64_t B, int64_t H, float scale, int64_t window,
+                   int64_t sinks, void* stream) {
+  g_last_error.clear();
+  tk::paged::Books b;
+  tk::paged::Pool pool;
+  if (int st = check_cache("tk_attn_decode", cache, &b, &pool)) return st;
+  if (layer < 0 || layer >= pool.layers)
+    return fail(TK_ERR_INVALID, "tk_attn_decode: layer %lld of %d", (long long)layer, pool.layers);
+  if (B < 0 || H <= 0 || H > (1 << 20) || H % cache->kv_heads)
+    return fail(TK_ERR_INVALID, "tk_attn_decode: B = %lld, H = %lld (a multiple of the cache's %lld heads)",
+                (long long)B, (long long)H, (long long)cache->kv_heads);
+  if (B == 0) return TK_OK;
+  if (q == nullptr || out == nullptr || (k_new == nullptr) != (v_new == nullptr))
+    return fail(TK_ERR_INVALID, "tk_attn_decode: null pointer");
+  if (slots == nullptr && B > cache->max_seqs)
+    return fail(TK_ERR_INVALID, "tk_attn_decode: %lld rows without slots, but %lld sequences", (long long)B,
+                (long long)cache->max_seqs);
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(TK_ERR_INVALID, "tk_attn_decode: scale must be positive");
+  if (window < 0 || sinks < 0 || window > (1ll << 31) - 1 || sinks > (1ll << 31) - 1)
+    return fail(TK_ERR_INVALID, "tk_attn_decode: negative or too large window or sinks");
+  if (q_stride_b % 2 || q_stride_h % 2 || q_stride_b < 0 || q_stride_h < 0 || !aligned(q, 4))
+    return fail(TK_ERR_INVALID, "tk_attn_decode: q needs even strides and a 4-byte aligned base");
+  if (k_new != nullptr && (new_stride_b % 8 || new_stride_h % 8 || new_stride_b < 0 || new_stride_h < 0 ||
+                           !aligned(k_new, 16) || !aligned(v_new, 16)))
+    return fail(TK_ERR_INVALID,
+                "tk_attn_decode: k_new/v_new need 16-byte aligned bases and strides (multiples of 8 elements)");
+  if (ld_out < H * cache->hd || ld_out % 2 || !aligned(out, 4))
+    return fail(TK_ERR_INVALID, "tk_attn_decode: out needs 4-byte aligned rows and ld_out >= H*hd");
+  const int64_t G = H / cache->kv_heads, gtiles = (G + tk::decode::kRows - 1) / tk::decode::kRows;
+  if (B * cache->kv_heads * gtiles > (1ll << 31) - 1)
+    return fail(TK_ERR_UNSUPPORTED, "tk_attn_decode: grid too large");
+  int dev;
+  DeviceInfo* info;
+  if (int st = current_device(&dev, &info)) return st;
+
+  tk::decode::Params p;
+  const int64_t hd = cache->hd, hd_k = hd < 16 ? 16 : hd, ps = cache->page_size;
+  p.q = static_cast<const __half*>(q);
+  p.k_new = static_cast<const __half*>(k_new);
+  p.v_new = static_cast<const __half*>(v_new);
+  p.head_stride = ps * hd;
+  p.page_stride = 2 * cache->kv_heads * p.head_stride;
+  p.k_pages = static_cast<__half*>(cache->pool) + layer * cache->num_pages * p.page_stride;
+  p.v_pages = p.k_pages + p.page_stride / 2;
+  p.table = b.table;
+  p.lens = b.lens;
+  p.slots = slots;
+  p.status = b.status;
+  p.out = static_cast<__half*>(out);
+  p.q_stride_b = q_stride_b;
+  p.q_stride_h = q_stride_h;
+  p.new_stride_b = new_stride_b;
+  p.new_stride_h = new_stride_h;
+  p.width = b.width;
+  p.ld_out = ld_out;
+  p.B = static_cast<int>(B);
+  p.H = static_cast<int>(H);
+  p.Hkv = static_cast<int>(cache->kv_heads);
+  p.G = static_cast<int>(G);
+  p.gtiles = static_cast<int>(gtiles);
+  p.max_seqs = b.max_seqs;
+  p.num_pages = b.num_pages;
+  p.page_shift = b.page_shift;
+  p.hd = static_cast<int>(hd);
+  p.window = static_cast<int>(window);
+  p.sinks = static_cast<int>(sinks);
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.wait_limit_ns = g_wait_limit_ns.load();
+  const int64_t keys = hd_k <= 32 ? 32 : 16;  // tk::decode::Cfg<HD>::KS
+  p.box_rows = static_cast<int>(std::min(keys, ps));
+  // pages as {hd, page_size, Hkv, P}; head_dim 8 as in tk_attn_fwd
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(ps),
+                        static_cast<cuuint64_t>(cache->kv_heads), static_cast<cuuint64_t>(cache->num_pages)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(hd) * 2, static_cast<cuuint64_t>(p.head_stride) * 2,
+                           static_cast<cuuint64_t>(p.page_stride) * 2};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(hd_k > 64 ? 64 : hd_k), static_cast<cuuint32_t>(p.box_rows), 1, 1};
+  const CUtensorMapSwizzle swz = hd_k >= 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                 : hd_k == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                              : CU_TENSOR_MAP_SWIZZLE_32B;
+  CUtensorMap mk, mv;
+  if (int st = make_map_f16(&mk, p.k_pages, 4, dims, strides, box, swz)) return st;
+  if (int st = make_map_f16(&mv, p.v_pages, 4, dims, strides, box, swz)) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool two = G > 8;
+  switch (hd_k) {
+    case 256: return two ? launch_decode<256, true>(info, 4, mk, mv, p, s) : launch_decode<256, false>(info, 4, mk, mv, p, s);
+    case 128: return two ? launch_decode<128, true>(info, 3, mk, mv, p, s) : launch_decode<128, false>(info, 3, mk, mv, p, s);
+    case 64: return two ? launch_decode<64, true>(info, 2, mk, mv, p, s) : launch_decode<64, false>(info, 2, mk, mv, p, s);
+    case 32: return two ? launch_decode<32, true>(info, 1, mk, mv, p, s) : launch_decode<32, false>(info, 1, mk, mv, p, s);
+    default: return two ? launch_decode<16, true>(info, 0, mk, mv, p, s) : launch_decode<16, false>(info, 0, mk, mv, p, s);
+  }
+}
+
 // ----------------------------------------------------------------------------
 int tk_peer_export(const void* ptr, void* handle, int64_t* offset) {
   g_last_error.clear();

@@ -28,6 +28,7 @@ enum DeviceError : unsigned {
   kDevOk = 0,
   kDevWaitTimeout = 1,   // an mbarrier wait exceeded the configured limit
   kDevBadShape = 2,      // a kernel saw an argument combination it cannot do
+  kDevCacheRefused = 3,  // a call on a paged cache did not apply (its status word says why)
 };
 
 struct ErrorWord {
