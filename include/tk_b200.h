@@ -179,6 +179,23 @@ TK_API int tk_attn_fwd(const void* q, const void* k, const void* v,
                 int64_t B, int64_t S, int64_t H, int64_t hd, float scale,
                 int causal, const int32_t* kv_len, void* stream);
 
+/* Causal attention with a sliding window. No counterpart in the reference,
+ * whose attention is causal or full (src/kernels.py:250-294). Query i sees key
+ * j when j <= i, j < kv_len[b], and i - j < window or j < sinks.
+ *   q    : fp16, logically [B, H, S, hd]; k, v: [B, Hkv, S, hd] with shared
+ *          strides, H % Hkv == 0 (query head h reads key-value head
+ *          h / (H / Hkv)); strides in elements, multiples of 8, contiguous last
+ *          dimension
+ *   out  : fp16 [B, S, H*hd], row stride ld_out (% 8 == 0); rows that see no
+ *          key are zero
+ *   kv_len : optional int32 [B]; keys and values at and past it may hold
+ *          anything
+ * window >= 1, sinks >= 0, scale > 0; hd in {8, 16, 32, 64, 128, 256}. */
+TK_API int tk_attn_window(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s, const void* k,
+                          const void* v, int64_t kv_stride_b, int64_t kv_stride_h, int64_t kv_stride_s, void* out,
+                          int64_t ld_out, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t hd, float scale,
+                          int64_t window, int64_t sinks, const int32_t* kv_len, void* stream);
+
 /* Whole-stack forward for small shapes, one launch: every layer of the
  * stack for one sequence per CTA (d_model = ffn = 128, 2 or 4 heads,
  * S <= 128; the harness's case 1 and the appendix shapes around it).

@@ -68,6 +68,8 @@ SIGNATURES = {
     "tk_gemm_tiles_set": (_I, [_I64, _I64, _I64, _I, _I]),
     "tk_gemm_tiles_clear": (_I, []),
     "tk_gemm_tiles_chosen": (_I, [_I64, _I64, _I64, _I]),
+    "tk_attn_window": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64,
+                            _F, _I64, _I64, _P, _P]),
     "tk_cache_reserve": (_I, [_C, _P, _P, _I64, _I, _P]),
     "tk_cache_fork": (_I, [_C, _P, _P, _I64, _P]),
     "tk_cache_release": (_I, [_C, _P, _I64, _P]),

@@ -71,18 +71,20 @@ def kernel_resources(ptxas_log: str) -> dict:
 
 
 def check_register_split(ptxas_log: str) -> None:
-    """The persistent attention kernel splits its launch allocation with
-    setmaxnreg (csrc/tk_attn.cuh kLaunchRegs): it must build with exactly
-    that many registers per thread, without spills and without a stack frame
-    (local memory would be reached through the reduced register budget)."""
+    """The persistent attention kernels (full and windowed) split their launch
+    allocation with setmaxnreg (csrc/tk_attn.cuh kLaunchRegs): they must build
+    with exactly that many registers per thread, without spills and without a
+    stack frame (local memory would be reached through the reduced register
+    budget)."""
     text = (HERE / "csrc" / "tk_attn.cuh").read_text()
     want = int(re.search(r"constexpr int kLaunchRegs = (\d+);", text).group(1))
-    found = {k: v for k, v in kernel_resources(ptxas_log).items() if "attn15attn_fwd_kernel" in k}
+    found = {k: v for k, v in kernel_resources(ptxas_log).items() if "attn15attn_fwd_kernel" in k
+             or "attn_window_kernel" in k}
     if not found:
         raise RuntimeError("ptxas output lists no attn_fwd_kernel")
     bad = {k: v for k, v in found.items() if v != (want, 0, 0)}
     if bad:
-        raise RuntimeError(f"attn_fwd_kernel needs {want} registers, no spills and no stack frame for its register "
+        raise RuntimeError(f"attn_fwd_kernel and attn_window_kernel need {want} registers, no spills and no stack frame for its register "
                            f"split; ptxas gave (registers, spill bytes, stack bytes) {sorted(bad.values())}")
 
 

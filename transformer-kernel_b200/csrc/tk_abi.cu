@@ -18,6 +18,7 @@
 #include "tk_attn.cuh"
 #include "tk_attn_decode.cuh"
 #include "tk_attn_wide.cuh"
+#include "tk_attn_window.cuh"
 #include "tk_gemm.cuh"
 #include "tk_layernorm.cuh"
 #include "tk_paged.cuh"
@@ -74,6 +75,11 @@ int cuda_fail(cudaError_t e, const char* what) {
               "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
 }
 
+int launched(cudaError_t e, const char* fn) {
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? TK_OK : cuda_fail(e, fn);
+}
+
 // --- driver entry point for cuTensorMapEncodeTiled (no -lcuda needed) --------
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -117,6 +123,7 @@ struct DeviceInfo {
   bool attn_attr_set[5] = {};
   bool small_attr_set[2] = {};
   bool decode_attr_set[5][2] = {};
+  bool window_attr_set[5] = {};
 };
 std::mutex g_dev_mu;
 DeviceInfo g_dev[64];
@@ -843,6 +850,132 @@ int tk_attn_fwd(const void* q, const void* k, const void* v, int64_t stride_b, i
 
 // ----------------------------------------------------------------------------
 // peer memory (CUDA IPC) and row copies
+}  // extern "C"
+
+namespace {
+
+// Tensor map of a logically [B, H, S, hd] fp16 tensor (strides in elements)
+// with boxes of 128 rows of one head. Dimensions go in increasing stride order
+// ({hd, H, S, B} or {hd, S, H, B}: *heads_inner); the stride of a dimension of
+// one entry means nothing and is replaced by one that fits. A null map only
+// checks the arguments.
+int map_bhsd(const char* fn, CUtensorMap* map, const void* base, int64_t B, int64_t H, int64_t S, int64_t hd,
+             int64_t sb, int64_t sh, int64_t ss, int* heads_inner) {
+  if (H == 1) sh = hd;
+  if (S == 1) ss = H * std::max(sh, hd);
+  if (B == 1) sb = std::max(H * sh, S * ss);
+  if (sb <= 0 || sh <= 0 || ss <= 0 || sb % 8 || sh % 8 || ss % 8 || !aligned(base, 16))
+    return fail(TK_ERR_INVALID, "%s: q/k/v need 16-byte aligned bases and positive strides (multiples of 8 elements)",
+                fn);
+  const bool inner = sh < ss;
+  const int64_t d1 = inner ? H : S, d2 = inner ? S : H, s1 = inner ? sh : ss, s2 = inner ? ss : sh;
+  if (s1 < hd || s2 < s1 * d1 || sb < s2)
+    return fail(TK_ERR_UNSUPPORTED, "%s: strides (b=%lld, h=%lld, s=%lld) overlap or are not batch-major", fn, (long long)sb, (long long)sh,
+                (long long)ss);
+  if (map == nullptr) return TK_OK;
+  const int64_t hd_k = hd < 16 ? 16 : hd;  // head_dim 8: TMA fills 8 columns with zeros
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(d1), static_cast<cuuint64_t>(d2),
+                        static_cast<cuuint64_t>(B)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(s1) * 2, static_cast<cuuint64_t>(s2) * 2,
+                           static_cast<cuuint64_t>(sb) * 2};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(hd_k > 64 ? 64 : hd_k), inner ? 1u : 128u, inner ? 128u : 1u, 1};
+  const CUtensorMapSwizzle swz = hd_k >= 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                 : hd_k == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                              : CU_TENSOR_MAP_SWIZZLE_32B;
+  *heads_inner = inner ? 1 : 0;
+  return make_map_f16(map, base, 4, dims, strides, box, swz);
+}
+
+template <int HD>
+int launch_window(DeviceInfo* info, int slot, const CUtensorMap (&maps)[3], const tk::attn::win::Params& p, bool small,
+                  cudaStream_t s) {
+  using C = tk::attn::win::Cfg<HD>;
+  auto kern = tk::attn::win::attn_window_kernel<HD>;
+  {
+    std::lock_guard<std::mutex> lk(g_dev_mu);
+    if (!info->window_attr_set[slot]) {
+      // as in tk_attn_fwd: the register split hands out exactly the launch allocation
+      cudaFuncAttributes fa;
+      cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes(window)");
+      if (fa.numRegs != tk::attn::kLaunchRegs)
+        return fail(TK_ERR_LAUNCH, "tk_attn_window: kernel built with %d registers per thread; its split needs %d",
+                    fa.numRegs, tk::attn::kLaunchRegs);
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(window smem)");
+      info->window_attr_set[slot] = true;
+    }
+  }
+  const int64_t q_tiles = (p.S + 127) / 128;
+  const int64_t items = static_cast<int64_t>(p.B) * p.H * ((q_tiles + C::GROUPS - 1) / C::GROUPS);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(items, info->sms));
+  return launched(launch(kern, dim3(grid), dim3(tk::attn::kThreads), C::SMEM_BYTES, s, small, maps[0], maps[1],
+                         maps[2], p),
+                  "tk_attn_window launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+int tk_attn_window(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s, const void* k,
+                   const void* v, int64_t kv_stride_b, int64_t kv_stride_h, int64_t kv_stride_s, void* out,
+                   int64_t ld_out, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t hd, float scale,
+                   int64_t window, int64_t sinks, const int32_t* kv_len, void* stream) {
+  g_last_error.clear();
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr)
+    return fail(TK_ERR_INVALID, "tk_attn_window: null pointer");
+  if (B <= 0 || S <= 0 || H <= 0 || Hkv <= 0 || hd <= 0 || H % Hkv)
+    return fail(TK_ERR_INVALID, "tk_attn_window: non-positive size, or H not a multiple of Hkv");
+  if (!tk_attn_supported(hd))
+    return fail(TK_ERR_UNSUPPORTED, "tk_attn_window: head_dim %lld not in {8,16,32,64,128,256}", (long long)hd);
+  if (window < 1 || sinks < 0)
+    return fail(TK_ERR_INVALID, "tk_attn_window: window must be at least 1 and sinks at least 0");
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(TK_ERR_INVALID, "tk_attn_window: scale must be positive");
+  if (ld_out < H * hd || ld_out % 8 || !aligned(out, 16))
+    return fail(TK_ERR_INVALID, "tk_attn_window: out needs 16-byte aligned rows and ld_out >= H*hd");
+  const int64_t q_tiles = (S + 127) / 128;
+  if (S > (1ll << 31) - 1024 || B * H > (1ll << 31) - 1 || B * H * q_tiles > (1ll << 31) - 1024)
+    return fail(TK_ERR_UNSUPPORTED, "tk_attn_window: grid too large");
+  tk::attn::win::Params p;
+  CUtensorMap maps[3];
+  if (int st = map_bhsd("tk_attn_window", nullptr, k, B, Hkv, S, hd, kv_stride_b, kv_stride_h, kv_stride_s, nullptr))
+    return st;
+  if (int st = map_bhsd("tk_attn_window", nullptr, v, B, Hkv, S, hd, kv_stride_b, kv_stride_h, kv_stride_s, nullptr))
+    return st;
+  if (int st = map_bhsd("tk_attn_window", &maps[0], q, B, H, S, hd, q_stride_b, q_stride_h, q_stride_s,
+                        &p.q_heads_inner))
+    return st;
+  if (int st = map_bhsd("tk_attn_window", &maps[1], k, B, Hkv, S, hd, kv_stride_b, kv_stride_h, kv_stride_s,
+                        &p.kv_heads_inner))
+    return st;
+  if (int st = map_bhsd("tk_attn_window", &maps[2], v, B, Hkv, S, hd, kv_stride_b, kv_stride_h, kv_stride_s,
+                        &p.kv_heads_inner))
+    return st;
+  int dev;
+  DeviceInfo* info;
+  if (int st = current_device(&dev, &info)) return st;
+  p.out = static_cast<__half*>(out);
+  p.ld_out = ld_out;
+  p.B = static_cast<int>(B);
+  p.S = static_cast<int>(S);
+  p.H = static_cast<int>(H);
+  p.G = static_cast<int>(H / Hkv);
+  p.window = static_cast<int>(std::min(window, S));
+  p.sinks = static_cast<int>(std::min(sinks, S));
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.kv_len = kv_len;
+  p.hd = static_cast<int>(hd);
+  p.wait_limit_ns = g_wait_limit_ns.load();
+  const bool small = static_cast<double>(B) * H * S * std::min(window + sinks, S) * hd <= kSmallAttnWork;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (hd == 256) return launch_window<256>(info, 4, maps, p, small, s);
+  if (hd == 128) return launch_window<128>(info, 3, maps, p, small, s);
+  if (hd == 64) return launch_window<64>(info, 2, maps, p, small, s);
+  if (hd == 32) return launch_window<32>(info, 1, maps, p, small, s);
+  return launch_window<16>(info, 0, maps, p, small, s);
+}
+
 // ----------------------------------------------------------------------------
 // paged key-value cache
 // ----------------------------------------------------------------------------
@@ -897,11 +1030,6 @@ int check_list(const char* fn, const int32_t* a, const int32_t* b, int64_t n) {
 
 size_t plan_smem(int64_t n, const tk::paged::Books& b) {
   return static_cast<size_t>(n) * 4 + static_cast<size_t>((b.max_seqs + 31) / 32) * 4;
-}
-
-int launched(cudaError_t e, const char* fn) {
-  if (e == cudaSuccess) e = cudaGetLastError();
-  return e == cudaSuccess ? TK_OK : cuda_fail(e, fn);
 }
 
 // The decode kernels: head_dim index and whether a tile holds more than eight query heads.

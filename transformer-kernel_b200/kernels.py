@@ -18,7 +18,7 @@ import torch
 
 import _tklib as tk
 
-__all__ = ["kernels_available", "attention_supported", "flash_attention"]
+__all__ = ["kernels_available", "attention_supported", "flash_attention", "window_attention"]
 
 
 def kernels_available() -> bool:
@@ -71,6 +71,57 @@ def flash_attention(
             q.stride(0), q.stride(1), q.stride(2),
             out.data_ptr(), out.stride(1),
             B, S, H, hd, float(scale), int(bool(causal)),
+            tk.ptr(kv_len), tk.stream_handle(dev),
+        )
+    return out
+
+
+def window_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    scale: float,
+    window: int,
+    sinks: int = 0,
+    kv_len: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Causal attention in which query i sees key j when ``i - j < window`` or
+    ``j < sinks``; returns the context in ``[B, S, H*hd]`` fp16.
+
+    ``q`` is ``[B, H, S, hd]``, ``k`` and ``v`` ``[B, Hkv, S, hd]`` with H a
+    multiple of Hkv (query head h reads head ``h // (H // Hkv)``), any strides
+    with a contiguous last dimension, shared by k and v. ``kv_len`` (int32
+    ``[B]``, optional) masks keys ``>= kv_len[b]``; what they hold is never
+    used. Rows that see no key are zero. The other values of k and v must be
+    finite: inside a tile a masked weight is 0 times the value. Backed by
+    ``tk_attn_window``; a window of S or more is plain causal attention."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or (q.shape[0], *q.shape[2:]) != (k.shape[0], *k.shape[2:]):
+        raise ValueError(f"q must be [B, H, S, hd] and k, v [B, Hkv, S, hd], got {q.shape}, {k.shape}, {v.shape}")
+    B, H, S, hd = q.shape
+    if q.numel() == 0 or k.numel() == 0 or H % k.shape[1] != 0:
+        raise ValueError(f"sizes must be positive and {H} query heads a multiple of {k.shape[1]} key-value heads")
+    if not (q.dtype == k.dtype == v.dtype == torch.float16):
+        raise tk.TKError("window_attention", -2, "q/k/v must be float16")
+    if k.stride() != v.stride() or q.stride(-1) != 1 or k.stride(-1) != 1:
+        raise tk.TKError("window_attention", -1, "k and v need identical strides, and all a contiguous last dimension")
+    dev = tk.require_cuda(q, k, v, kv_len, out)
+    if out is None:
+        out = torch.empty((B, S, H * hd), dtype=torch.float16, device=dev)
+    elif (out.shape != (B, S, H * hd) or out.dtype != torch.float16 or out.stride(-1) != 1
+          or (B > 1 and out.stride(0) != S * out.stride(1))):
+        raise ValueError("out must be fp16 [B, S, H*hd] with unit last stride and rows S*ld apart per batch")
+    if kv_len is not None:
+        if kv_len.shape != (B,):
+            raise ValueError(f"kv_len must have shape ({B},), got {tuple(kv_len.shape)}")
+        kv_len = kv_len.to(dtype=torch.int32).contiguous()
+    with torch.cuda.device(dev):
+        tk.call(
+            "tk_attn_window",
+            q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
+            k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
+            out.data_ptr(), out.stride(1) if S > 1 else max(out.stride(1), H * hd),
+            B, S, H, k.shape[1], hd, float(scale), int(window), int(sinks),
             tk.ptr(kv_len), tk.stream_handle(dev),
         )
     return out
