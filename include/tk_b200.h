@@ -285,7 +285,8 @@ typedef enum tk_cache_status {
   TK_CACHE_BAD_SLOT = 2,      /* slot out of range or twice, or a negative count  */
   TK_CACHE_TOO_LONG = 4,      /* longer than the slot's row of the page table     */
   TK_CACHE_BAD_PAGE = 8,      /* the page table names a page outside the pool     */
-  TK_CACHE_NOT_EMPTY = 16     /* a slot that has to be empty is not               */
+  TK_CACHE_NOT_EMPTY = 16,    /* a slot that has to be empty is not               */
+  TK_CACHE_TIMED_OUT = 32     /* a wait inside an attention call gave up          */
 } tk_cache_status;
 
 /* Sequence slots[i] grows by counts[i] tokens and takes the pages that they
@@ -326,11 +327,20 @@ TK_API int tk_cache_store(const tk_cache* cache, int64_t layer, const void* k, c
  *                  row b is sequence b. Rows with slot -1 are left untouched
  *   out          : fp16 [B, H*hd], row stride ld_out
  * An empty sequence gives zeros. Positions past seq_len and hidden keys may
- * hold anything. hd in {8, 16, 32, 64, 128, 256}; scale > 0. */
+ * hold anything. hd in {8, 16, 32, 64, 128, 256}; scale > 0.
+ *   max_len   : 0, or a bound on the rows' lengths where the host knows a
+ *               smaller one than the page table's width; it only helps to
+ *               choose how the work is divided
+ *   workspace : NULL, or at least tk_attn_decode_workspace_bytes(hd) bytes
+ *               (for the current device; negative on error), 256-byte
+ *               aligned, contents irrelevant, not shared by calls that
+ *               overlap on the GPU. With it long caches are split over the
+ *               whole GPU instead of one CTA per row and key-value head. */
+TK_API int64_t tk_attn_decode_workspace_bytes(int64_t hd);
 TK_API int tk_attn_decode(const tk_cache* cache, int64_t layer, const void* q, int64_t q_stride_b, int64_t q_stride_h,
                           const void* k_new, const void* v_new, int64_t new_stride_b, int64_t new_stride_h,
                           const int32_t* slots, void* out, int64_t ld_out, int64_t B, int64_t H, float scale,
-                          int64_t window, int64_t sinks, void* stream);
+                          int64_t window, int64_t sinks, int64_t max_len, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Guard probes, same meaning as the reference's can_fuse
  * (src/fused_kernels.py:62-64) and attention_supported

@@ -110,7 +110,7 @@ def ints(*values):
 # refusals that need no device
 # ---------------------------------------------------------------------------
 def test_status_names_every_bit_of_the_header():
-    assert sorted(paged_cache.STATUS) == [1, 2, 4, 8, 16]
+    assert sorted(paged_cache.STATUS) == [1, 2, 4, 8, 16, 32]
 
 
 @pytest.mark.parametrize("change, error", [
@@ -150,10 +150,11 @@ def test_c_entries_refuse_on_host():
     assert lib.tk_cache_store(ok, 0, 8, 16, 64, 64, 64, 16, None, 1, 4, None) == -1
     assert lib.tk_cache_store(ok, 0, None, 16, 64, 64, 64, 16, None, 1, 4, None) == -1
     # decode: layer, heads, lone k_new, rows without slots, scale, window, strides, out
-    def dec(layer=0, qs=64, k=16, v=16, kvs=64, slots=16, ld=256, B=1, H=4, scale=1.0, w=0, s=0):
-        return lib.tk_attn_decode(ok, layer, 16, 4 * qs, qs, k, v, 2 * kvs, kvs, slots, 16, ld, B, H, scale, w, s, None)
+    def dec(layer=0, qs=64, k=16, v=16, kvs=64, slots=16, ld=256, B=1, H=4, scale=1.0, w=0, s=0, m=0):
+        return lib.tk_attn_decode(ok, layer, 16, 4 * qs, qs, k, v, 2 * kvs, kvs, slots, 16, ld, B, H, scale, w, s,
+                                  m, None, 0, None)
     for kw in (dict(layer=-1), dict(H=3), dict(H=0), dict(v=None), dict(slots=None, B=9), dict(scale=0.0),
-               dict(scale=float("nan")), dict(scale=-1.0), dict(w=-1), dict(s=-1), dict(qs=63), dict(kvs=60),
+               dict(scale=float("nan")), dict(scale=-1.0), dict(w=-1), dict(s=-1), dict(m=-1), dict(qs=63), dict(kvs=60),
                dict(ld=255), dict(ld=128)):
         assert dec(**kw) == -1, kw
 
@@ -515,6 +516,45 @@ def test_decode_long_and_ragged(cuda_device):
     cache, kv, g = filled([5000, 1, 20011, 777], 64, 2, 64)
     check_decode(cache, kv, g, 8)
     check_decode(cache, kv, g, 8, window=4096, sinks=17)
+
+
+def run_each_way(cache, call):
+    """The output of ``call(max_len)`` for bounds that make the library give a
+    segment a warp or a CTA, and for none (wide tables: split over the GPU)."""
+    return [call(m).clone() for m in (1, 2047, 4096, 0)]
+
+
+@gpu
+@pytest.mark.parametrize("head_dim", [8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("kv_heads, heads", [(16, 16), (3, 36)])
+def test_decode_every_division_of_the_work(cuda_device, head_dim, kv_heads, heads):
+    """Tables wide enough that the calls are split; with bounds on the
+    lengths the same rows run by a warp or a CTA each. Sequences shorter than
+    a step, empty ones, one that spans many CTAs, padding between them."""
+    lens = [3, 0, 1500, 1, 40, 33, 0, 700, 64, 16, 2500] + [17] * 21
+    cache, kv, g = filled(lens, 16, kv_heads, head_dim, width=300)
+    for window, sinks in ((0, 0), (600, 20)):
+        check_decode(cache, kv, g, heads, window=window, sinks=sinks)
+        check_decode(cache, kv, g, heads, window=window, sinks=sinks, rows=[10, -1, 0, 1, 2, -1, 7])
+    q = torch.randn(len(lens), heads, head_dim, generator=g, device="cuda").half()
+    scale = head_dim ** -0.5
+    outs = run_each_way(cache, lambda m: cache.attend(0, q, scale, max_len=m))
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert not any(o[b].any() for o in outs)
+            continue
+        ref, tol = attend_reference(q[b], kv[b][0], kv[b][1], scale)
+        for o in outs:
+            assert bool(((o[b].view(heads, head_dim).double() - ref).abs() <= tol).all())
+
+
+@gpu
+def test_decode_one_long_sequence_over_the_whole_gpu(cuda_device):
+    """One key-value head, 50,000 keys: hundreds of parts joined in order."""
+    cache, kv, g = filled([50000], 64, 1, 64)
+    check_decode(cache, kv, g, 8)
+    cache, kv, g = filled([1, 30000, 2], 128, 1, 256)
+    check_decode(cache, kv, g, 20)
 
 
 @gpu

@@ -78,7 +78,8 @@ SIGNATURES = {
     "tk_cache_rebuild": (_I, [_C, _P]),
     "tk_cache_store": (_I, [_C, _I64, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _P]),
     "tk_attn_decode": (_I, [_C, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _F, _I64, _I64,
-                            _P]),
+                            _I64, _P, _I64, _P]),
+    "tk_attn_decode_workspace_bytes": (_I64, [_I64]),
     "tk_peer_export": (_I, [_P, _P, ctypes.POINTER(ctypes.c_int64)]),
     "tk_peer_import": (_I, [_P, _I64, ctypes.POINTER(ctypes.c_void_p)]),
     "tk_peer_release": (_I, [_P]),

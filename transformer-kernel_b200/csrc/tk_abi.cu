@@ -1032,23 +1032,75 @@ size_t plan_smem(int64_t n, const tk::paged::Books& b) {
   return static_cast<size_t>(n) * 4 + static_cast<size_t>((b.max_seqs + 31) / 32) * 4;
 }
 
-// The decode kernels: head_dim index and whether a tile holds more than eight query heads.
+// Workspace of the split decode kernel: what happens to each segment, then
+// per CTA two parts (maximum and sum, O).
+constexpr int64_t kMaxSegments = 65536;
+
+// How a decode call divides its segments (row, key-value head, 16 query heads).
+enum { kWarpEach, kCtaEach, kSplit };
+
+template <int HD>
+int64_t split_bytes(int sms) {
+  const int64_t parts = 2ll * sms * tk::decode::Cfg<HD>::CTAS;
+  return kMaxSegments * 8 + parts * tk::decode::kRows * (2 + HD) * 4;
+}
+
 template <int HD, bool TWO>
-int launch_decode(DeviceInfo* info, int slot, const CUtensorMap& mk, const CUtensorMap& mv,
-                  const tk::decode::Params& p, cudaStream_t s) {
-  auto kern = tk::decode::decode_kernel<HD, TWO>;
+int launch_decode(DeviceInfo* info, int slot, tk::decode::Params& p, int64_t page_size, int how, void* workspace,
+                  int64_t workspace_bytes, cudaStream_t s) {
+  using C = tk::decode::Cfg<HD>;
+  // pages as {hd, page_size, Hkv, P}; head_dim 8 as in tk_attn_fwd. Boxes never cross a page
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.hd), static_cast<cuuint64_t>(page_size),
+                        static_cast<cuuint64_t>(p.Hkv), static_cast<cuuint64_t>(p.num_pages)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(p.hd) * 2, static_cast<cuuint64_t>(p.head_stride) * 2,
+                           static_cast<cuuint64_t>(p.page_stride) * 2};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(C::COLS),
+                       static_cast<cuuint32_t>(std::min<int64_t>(C::KS, page_size)), 1, 1};
+  const CUtensorMapSwizzle swz = C::SPAN == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                 : C::SPAN == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                 : CU_TENSOR_MAP_SWIZZLE_32B;
+  CUtensorMap mk, mv;
+  if (int st = make_map_f16(&mk, p.k_pages, 4, dims, strides, box, swz)) return st;
+  if (int st = make_map_f16(&mv, p.v_pages, 4, dims, strides, box, swz)) return st;
   {
     std::lock_guard<std::mutex> lk(g_dev_mu);
     if (!info->decode_attr_set[slot][TWO]) {
-      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           tk::decode::Cfg<HD>::SMEM_BYTES);
+      cudaError_t e = cudaFuncSetAttribute(tk::decode::decode_kernel<HD, TWO, 4>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(tk::decode::decode_kernel<HD, TWO, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 C::SMEM_BYTES);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(tk::decode::decode_split_kernel<HD, TWO>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
       if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(decode smem)");
       info->decode_attr_set[slot][TWO] = true;
     }
   }
-  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(p.B) * p.Hkv * p.gtiles);
-  return launched(launch(kern, dim3(grid), dim3(tk::decode::kThreads), tk::decode::Cfg<HD>::SMEM_BYTES, s, true, mk,
-                         mv, p),
+  const int64_t segments = static_cast<int64_t>(p.B) * p.Hkv * p.gtiles;
+  if (how == kWarpEach)
+    return launched(launch(tk::decode::decode_kernel<HD, TWO, 1>, dim3(static_cast<unsigned>((segments + 3) / 4)),
+                           dim3(tk::decode::kThreads), C::SMEM_BYTES, s, true, mk, mv, p),
+                    "tk_attn_decode launch");
+  if (how == kCtaEach)
+    return launched(launch(tk::decode::decode_kernel<HD, TWO, 4>, dim3(static_cast<unsigned>(segments)),
+                           dim3(tk::decode::kThreads), C::SMEM_BYTES, s, true, mk, mv, p),
+                    "tk_attn_decode launch");
+  if (workspace_bytes < split_bytes<HD>(info->sms))
+    return fail(TK_ERR_INVALID, "tk_attn_decode: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                (long long)split_bytes<HD>(info->sms));
+  const int grid = info->sms * C::CTAS;
+  p.ctas = grid;
+  p.info = static_cast<int2*>(workspace);
+  p.part_ml = reinterpret_cast<float*>(p.info + kMaxSegments);
+  p.part_o = p.part_ml + 2ll * p.ctas * 2 * tk::decode::kRows;
+  if (int st = launched(launch(tk::decode::decode_split_kernel<HD, TWO>, dim3(grid), dim3(tk::decode::kThreads),
+                               C::SMEM_BYTES, s, true, mk, mv, p),
+                        "tk_attn_decode launch"))
+    return st;
+  const int rows = std::min(p.G, tk::decode::kRows);
+  return launched(launch(tk::decode::join_kernel<HD>, dim3(static_cast<unsigned>(segments), rows),
+                         dim3(segments * rows <= 2 * info->sms ? tk::decode::kJoinThreads : 256), 0, s, true, p),
                   "tk_attn_decode launch");
 }
 
@@ -1202,7 +1254,7 @@ int tk_cache_store(const tk_cache* cache, int64_t layer, const void* k, const vo
 int tk_attn_decode(const tk_cache* cache, int64_t layer, const void* q, int64_t q_stride_b, int64_t q_stride_h,
                    const void* k_new, const void* v_new, int64_t new_stride_b, int64_t new_stride_h,
                    const int32_t* slots, void* out, int64_t ld_out, int64_t B, int64_t H, float scale, int64_t window,
-                   int64_t sinks, void* stream) {
+                   int64_t sinks, int64_t max_len, void* workspace, int64_t workspace_bytes, void* stream) {
   g_last_error.clear();
   tk::paged::Books b;
   tk::paged::Pool pool;
@@ -1219,8 +1271,8 @@ int tk_attn_decode(const tk_cache* cache, int64_t layer, const void* q, int64_t 
     return fail(TK_ERR_INVALID, "tk_attn_decode: %lld rows without slots, but %lld sequences", (long long)B,
                 (long long)cache->max_seqs);
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail(TK_ERR_INVALID, "tk_attn_decode: scale must be positive");
-  if (window < 0 || sinks < 0 || window > (1ll << 31) - 1 || sinks > (1ll << 31) - 1)
-    return fail(TK_ERR_INVALID, "tk_attn_decode: negative or too large window or sinks");
+  if (window < 0 || sinks < 0 || max_len < 0 || window > (1ll << 31) - 1 || sinks > (1ll << 31) - 1)
+    return fail(TK_ERR_INVALID, "tk_attn_decode: negative or too large window, sinks or max_len");
   if (q_stride_b % 2 || q_stride_h % 2 || q_stride_b < 0 || q_stride_h < 0 || !aligned(q, 4))
     return fail(TK_ERR_INVALID, "tk_attn_decode: q needs even strides and a 4-byte aligned base");
   if (k_new != nullptr && (new_stride_b % 8 || new_stride_h % 8 || new_stride_b < 0 || new_stride_h < 0 ||
@@ -1237,7 +1289,7 @@ int tk_attn_decode(const tk_cache* cache, int64_t layer, const void* q, int64_t 
   if (int st = current_device(&dev, &info)) return st;
 
   tk::decode::Params p;
-  const int64_t hd = cache->hd, hd_k = hd < 16 ? 16 : hd, ps = cache->page_size;
+  const int64_t hd = cache->hd, ps = cache->page_size;
   p.q = static_cast<const __half*>(q);
   p.k_new = static_cast<const __half*>(k_new);
   p.v_new = static_cast<const __half*>(v_new);
@@ -1269,28 +1321,53 @@ int tk_attn_decode(const tk_cache* cache, int64_t layer, const void* q, int64_t 
   p.sinks = static_cast<int>(sinks);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.wait_limit_ns = g_wait_limit_ns.load();
-  const int64_t keys = hd_k <= 32 ? 32 : 16;  // tk::decode::Cfg<HD>::KS
-  p.box_rows = static_cast<int>(std::min(keys, ps));
-  // pages as {hd, page_size, Hkv, P}; head_dim 8 as in tk_attn_fwd
-  cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(ps),
-                        static_cast<cuuint64_t>(cache->kv_heads), static_cast<cuuint64_t>(cache->num_pages)};
-  cuuint64_t strides[3] = {static_cast<cuuint64_t>(hd) * 2, static_cast<cuuint64_t>(p.head_stride) * 2,
-                           static_cast<cuuint64_t>(p.page_stride) * 2};
-  cuuint32_t box[4] = {static_cast<cuuint32_t>(hd_k > 64 ? 64 : hd_k), static_cast<cuuint32_t>(p.box_rows), 1, 1};
-  const CUtensorMapSwizzle swz = hd_k >= 64   ? CU_TENSOR_MAP_SWIZZLE_128B
-                                 : hd_k == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                              : CU_TENSOR_MAP_SWIZZLE_32B;
-  CUtensorMap mk, mv;
-  if (int st = make_map_f16(&mk, p.k_pages, 4, dims, strides, box, swz)) return st;
-  if (int st = make_map_f16(&mv, p.v_pages, 4, dims, strides, box, swz)) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool two = G > 8;
-  switch (hd_k) {
-    case 256: return two ? launch_decode<256, true>(info, 4, mk, mv, p, s) : launch_decode<256, false>(info, 4, mk, mv, p, s);
-    case 128: return two ? launch_decode<128, true>(info, 3, mk, mv, p, s) : launch_decode<128, false>(info, 3, mk, mv, p, s);
-    case 64: return two ? launch_decode<64, true>(info, 2, mk, mv, p, s) : launch_decode<64, false>(info, 2, mk, mv, p, s);
-    case 32: return two ? launch_decode<32, true>(info, 1, mk, mv, p, s) : launch_decode<32, false>(info, 1, mk, mv, p, s);
-    default: return two ? launch_decode<16, true>(info, 0, mk, mv, p, s) : launch_decode<16, false>(info, 0, mk, mv, p, s);
+  // Most keys that a row may see, as far as the host knows: the caller's
+  // bound on the lengths, or the table's width; and the window's.
+  int64_t span = max_len > 0 ? std::min<int64_t>(max_len, b.width * ps) : b.width * ps;
+  if (window > 0) span = std::min<int64_t>(span, window + sinks);
+  const int64_t segments = B * p.Hkv * gtiles;
+  const bool can_split = workspace != nullptr && B <= tk::decode::kMaxRows && segments <= kMaxSegments;
+  // Few segments over long caches, and any number over so long ones that one
+  // straggler would cost more than an uneven grid, are split over the GPU (8
+  // groups of hd 128 x 4096 keys: 11 us against 33 by a CTA each; 64 groups:
+  // 32 against 36; 128 heads of hd 64 x 1024: 14 against 9, so not below 2048
+  // keys). Many short ones get a warp each, without a merge (1024 heads of hd
+  // 64 x 64 keys: 5 us against 11, x 256: 10 against 15; 128 heads: 8 against
+  // 4.5), the others a CTA.
+  int how = kCtaEach;
+  if (can_split && (span > 4096 || (span >= 2048 && segments < info->sms))) how = kSplit;
+  else if (segments >= 3 * info->sms && span <= 2048) how = kWarpEach;
+  p.min_steps = 8;
+  if (how == kSplit && !aligned(workspace, 256))
+    return fail(TK_ERR_INVALID, "tk_attn_decode: the workspace needs 256-byte alignment");
+  auto run = [&](auto launch_two, auto launch_one, int slot) {
+    return (two ? launch_two : launch_one)(info, slot, p, ps, how, workspace, workspace_bytes, s);
+  };
+  switch (hd) {
+    case 256: return run(launch_decode<256, true>, launch_decode<256, false>, 4);
+    case 128: return run(launch_decode<128, true>, launch_decode<128, false>, 3);
+    case 64: return run(launch_decode<64, true>, launch_decode<64, false>, 2);
+    case 32: return run(launch_decode<32, true>, launch_decode<32, false>, 1);
+    default: return run(launch_decode<16, true>, launch_decode<16, false>, 0);
+  }
+}
+
+int64_t tk_attn_decode_workspace_bytes(int64_t hd) {
+  g_last_error.clear();
+  int dev;
+  DeviceInfo* info;
+  if (!tk_attn_supported(hd))
+    return fail(TK_ERR_UNSUPPORTED, "tk_attn_decode_workspace_bytes: head_dim %lld not in {8,16,32,64,128,256}",
+                (long long)hd);
+  if (int st = current_device(&dev, &info)) return st;
+  switch (hd) {
+    case 256: return split_bytes<256>(info->sms);
+    case 128: return split_bytes<128>(info->sms);
+    case 64: return split_bytes<64>(info->sms);
+    case 32: return split_bytes<32>(info->sms);
+    default: return split_bytes<16>(info->sms);
   }
 }
 

@@ -34,6 +34,7 @@ enum : int {
   kTooLong = 4,     // a sequence longer than its row of the page table
   kBadPage = 8,     // the page table names a page outside the pool
   kNotEmpty = 16,   // a slot that has to be empty is not
+  kTimedOut = 32,   // a wait inside an attention call gave up
 };
 
 struct Books {

@@ -46,6 +46,7 @@ STATUS = {
     4: "a sequence is longer than its row of the page table, or has fewer tokens than the call stores",
     8: "the page table names a page outside the pool",
     16: "a slot that has to be empty holds a sequence",
+    32: "a device wait gave up",
 }
 
 Slots = Union[torch.Tensor, Sequence[int]]
@@ -113,6 +114,11 @@ class PagedCache:
         self.page_table = page_table.view(max_seqs, max_pages_per_seq)
         self.status, self.live_pages = status[0], live[0]
         self._scratch = torch.empty(3 * num_pages + 1, dtype=torch.int32, device=self.device)
+        with torch.cuda.device(self.device):
+            need = tk.lib().tk_attn_decode_workspace_bytes(self.head_dim)
+        if need < 0:
+            raise tk.TKError("PagedCache", need, tk.lib().tk_last_error().decode(errors="replace"))
+        self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
         self._c = tk.Cache(
             page_table.data_ptr(), self.seq_lens.data_ptr(), self.ref_counts.data_ptr(), mask.data_ptr(),
             status.data_ptr(), live.data_ptr(), self._scratch.data_ptr(), pages.data_ptr(), max_seqs,
@@ -229,6 +235,7 @@ class PagedCache:
         slots: Optional[Slots] = None,
         window: int = 0,
         sinks: int = 0,
+        max_len: int = 0,
         out: Optional[torch.Tensor] = None,
     ) -> torch.Tensor:
         """Attention of one new token per row, the last of its sequence;
@@ -263,7 +270,8 @@ class PagedCache:
         tk.require_cuda(self.pages, out)
         self._call("tk_attn_decode", int(layer), q.data_ptr(), *_strides(q)[:2], tk.ptr(k_new), tk.ptr(v_new),
                    *((0, 0) if k_new is None else _strides(k_new)[:2]), tk.ptr(s),
-                   out.data_ptr(), max(out.stride(0), H * hd), B, H, float(scale), int(window), int(sinks))
+                   out.data_ptr(), max(out.stride(0), H * hd), B, H, float(scale), int(window), int(sinks), int(max_len),
+                   self._workspace.data_ptr(), self._workspace.numel())
         return out
 
     # -- helpers ---------------------------------------------------------------------
