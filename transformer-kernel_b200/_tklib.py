@@ -117,7 +117,7 @@ def lib() -> ctypes.CDLL:
 
 
 def call(name: str, *args) -> int:
-    status = getattr(lib(), name)(*args)
+    status = getattr(_lib or lib(), name)(*args)
     if status != TK_OK:
         raise TKError(name, status, lib().tk_last_error().decode(errors="replace"))
     return status
@@ -136,7 +136,19 @@ def dtype_code(dt: torch.dtype) -> int:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """cudaStream_t of the device's current stream (the raw handle, without
+    the torch.cuda.Stream object around it, which costs 2 us a call)."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def call_on(device: torch.device, name: str, *args) -> int:
+    """``call`` on the device's current stream (the last argument of every
+    launching entry), with the device current during the call."""
+    if torch.cuda.current_device() == device.index:
+        return call(name, *args, stream_handle(device))
+    with torch.cuda.device(device):
+        return call(name, *args, stream_handle(device))
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:

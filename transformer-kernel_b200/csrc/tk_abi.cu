@@ -1225,6 +1225,9 @@ int tk_cache_store(const tk_cache* cache, int64_t layer, const void* k, const vo
   if (S < 0 || S > (1ll << 31) - 1) return fail(TK_ERR_INVALID, "tk_cache_store: S = %lld", (long long)S);
   if (B == 0 || S == 0) return TK_OK;
   if (k == nullptr || v == nullptr) return fail(TK_ERR_INVALID, "tk_cache_store: null pointer");
+  if (B == 1) stride_b = 0;  // the stride of a dimension of one entry means nothing
+  if (cache->kv_heads == 1) stride_h = 0;
+  if (S == 1) stride_s = 0;
   if (stride_b % 8 || stride_h % 8 || stride_s % 8 || stride_b < 0 || stride_h < 0 || stride_s < 0 ||
       !aligned(k, 16) || !aligned(v, 16))
     return fail(TK_ERR_INVALID, "tk_cache_store: k/v need 16-byte aligned bases and strides (multiples of 8)");
@@ -1265,6 +1268,9 @@ int tk_attn_decode(const tk_cache* cache, int64_t layer, const void* q, int64_t 
     return fail(TK_ERR_INVALID, "tk_attn_decode: B = %lld, H = %lld (a multiple of the cache's %lld heads)",
                 (long long)B, (long long)H, (long long)cache->kv_heads);
   if (B == 0) return TK_OK;
+  if (B == 1) q_stride_b = new_stride_b = 0;  // the stride of a dimension of one entry means nothing
+  if (H == 1) q_stride_h = 0;
+  if (cache->kv_heads == 1) new_stride_h = 0;
   if (q == nullptr || out == nullptr || (k_new == nullptr) != (v_new == nullptr))
     return fail(TK_ERR_INVALID, "tk_attn_decode: null pointer");
   if (slots == nullptr && B > cache->max_seqs)

@@ -96,32 +96,32 @@ def window_attention(
     used. Rows that see no key are zero. The other values of k and v must be
     finite: inside a tile a masked weight is 0 times the value. Backed by
     ``tk_attn_window``; a window of S or more is plain causal attention."""
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or (q.shape[0], *q.shape[2:]) != (k.shape[0], *k.shape[2:]):
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError(f"q must be [B, H, S, hd] and k, v [B, Hkv, S, hd], got {q.shape}, {k.shape}, {v.shape}")
     B, H, S, hd = q.shape
-    if q.numel() == 0 or k.numel() == 0 or H % k.shape[1] != 0:
-        raise ValueError(f"sizes must be positive and {H} query heads a multiple of {k.shape[1]} key-value heads")
+    Bk, Hkv, Sk, hdk = k.shape
+    if (B, S, hd) != (Bk, Sk, hdk):
+        raise ValueError(f"q must be [B, H, S, hd] and k, v [B, Hkv, S, hd], got {q.shape}, {k.shape}, {v.shape}")
+    if B * H * S * hd * Hkv == 0 or H % Hkv != 0:
+        raise ValueError(f"sizes must be positive and {H} query heads a multiple of {Hkv} key-value heads")
     if not (q.dtype == k.dtype == v.dtype == torch.float16):
         raise tk.TKError("window_attention", -2, "q/k/v must be float16")
-    if k.stride() != v.stride() or q.stride(-1) != 1 or k.stride(-1) != 1:
+    qs, ks = q.stride(), k.stride()
+    if ks != v.stride() or qs[3] != 1 or ks[3] != 1:
         raise tk.TKError("window_attention", -1, "k and v need identical strides, and all a contiguous last dimension")
     dev = tk.require_cuda(q, k, v, kv_len, out)
     if out is None:
         out = torch.empty((B, S, H * hd), dtype=torch.float16, device=dev)
-    elif (out.shape != (B, S, H * hd) or out.dtype != torch.float16 or out.stride(-1) != 1
-          or (B > 1 and out.stride(0) != S * out.stride(1))):
-        raise ValueError("out must be fp16 [B, S, H*hd] with unit last stride and rows S*ld apart per batch")
+        ld = H * hd
+    else:
+        ld = out.stride(1) if S > 1 else max(out.stride(1), H * hd)
+        if (out.shape != (B, S, H * hd) or out.dtype != torch.float16 or out.stride(2) != 1
+                or (B > 1 and out.stride(0) != S * ld)):
+            raise ValueError("out must be fp16 [B, S, H*hd] with unit last stride and rows S*ld apart per batch")
     if kv_len is not None:
         if kv_len.shape != (B,):
             raise ValueError(f"kv_len must have shape ({B},), got {tuple(kv_len.shape)}")
         kv_len = kv_len.to(dtype=torch.int32).contiguous()
-    with torch.cuda.device(dev):
-        tk.call(
-            "tk_attn_window",
-            q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
-            k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-            out.data_ptr(), out.stride(1) if S > 1 else max(out.stride(1), H * hd),
-            B, S, H, k.shape[1], hd, float(scale), int(window), int(sinks),
-            tk.ptr(kv_len), tk.stream_handle(dev),
-        )
+    tk.call_on(dev, "tk_attn_window", q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), v.data_ptr(), ks[0], ks[1],
+               ks[2], out.data_ptr(), ld, B, S, H, Hkv, hd, float(scale), int(window), int(sinks), tk.ptr(kv_len))
     return out

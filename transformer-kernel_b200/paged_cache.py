@@ -123,6 +123,8 @@ class PagedCache:
             page_table.data_ptr(), self.seq_lens.data_ptr(), self.ref_counts.data_ptr(), mask.data_ptr(),
             status.data_ptr(), live.data_ptr(), self._scratch.data_ptr(), pages.data_ptr(), max_seqs,
             max_pages_per_seq, num_pages, page_size, num_layers, kv_heads, head_dim)
+        self._handle = ctypes.byref(self._c)
+        self._workspace_ptr, self._workspace_bytes = self._workspace.data_ptr(), need
         self.reset()
 
     # -- the books as a whole ---------------------------------------------------
@@ -222,7 +224,7 @@ class PagedCache:
         if s.numel() != k.shape[0] or (c is not None and c.numel() != k.shape[0]):
             raise ValueError(f"{k.shape[0]} rows, but {s.numel()} slots"
                              + ("" if c is None else f" and {c.numel()} counts"))
-        self._call("tk_cache_store", int(layer), k.data_ptr(), v.data_ptr(), *_strides(k)[:3],
+        self._call("tk_cache_store", int(layer), k.data_ptr(), v.data_ptr(), *k.stride()[:3],
                    s.data_ptr(), tk.ptr(c), k.shape[0], k.shape[2])
 
     def attend(
@@ -248,45 +250,54 @@ class PagedCache:
         keys that lie ``window`` or more tokens back, except the first
         ``sinks``. Without ``slots`` row b is sequence b; rows with slot -1
         are left as they are, an empty sequence gives zeros."""
-        if q.dim() != 3 or q.shape[2] != self.head_dim or q.shape[1] == 0 or q.shape[1] % self.kv_heads:
-            raise ValueError(f"q must be [B, a multiple of {self.kv_heads} heads, {self.head_dim}], got "
-                             f"{tuple(q.shape)}")
-        if (k_new is None) != (v_new is None):
-            raise ValueError("k_new and v_new come together")
-        B, H, hd = q.shape
-        if k_new is not None and not (k_new.shape == v_new.shape == (B, self.kv_heads, hd)):
-            raise ValueError(f"k_new/v_new must be {(B, self.kv_heads, hd)}, got {tuple(k_new.shape)} and "
-                             f"{tuple(v_new.shape)}")
+        K, hd = self.kv_heads, self.head_dim
+        shape = q.shape
+        if len(shape) != 3 or shape[2] != hd or shape[1] == 0 or shape[1] % K:
+            raise ValueError(f"q must be [B, a multiple of {K} heads, {hd}], got {tuple(shape)}")
+        B, H, _ = shape
         self._check_data("attend", q)
-        if k_new is not None:
+        qs = q.stride()
+        new = (None, None, 0, 0)
+        if k_new is not None and v_new is not None:
+            if not (k_new.shape == v_new.shape == (B, K, hd)):
+                raise ValueError(f"k_new/v_new must be {(B, K, hd)}, got {tuple(k_new.shape)} and "
+                                 f"{tuple(v_new.shape)}")
             self._check_data("attend", k_new, v_new)
+            ns = k_new.stride()
+            new = (k_new.data_ptr(), v_new.data_ptr(), ns[0], ns[1])
+        elif k_new is not None or v_new is not None:
+            raise ValueError("k_new and v_new come together")
         if out is None:
             out = torch.empty((B, H * hd), dtype=torch.float16, device=self.device)
-        elif out.shape != (B, H * hd) or out.dtype != torch.float16 or (out.stride(1) != 1 and out.numel() > 0):
-            raise ValueError(f"out must be fp16 {(B, H * hd)} with a contiguous last dimension")
-        s = None if slots is None else self._slots(slots)
-        if s is not None and s.numel() != B:
-            raise ValueError(f"{B} rows, but {s.numel()} slots")
-        tk.require_cuda(self.pages, out)
-        self._call("tk_attn_decode", int(layer), q.data_ptr(), *_strides(q)[:2], tk.ptr(k_new), tk.ptr(v_new),
-                   *((0, 0) if k_new is None else _strides(k_new)[:2]), tk.ptr(s),
-                   out.data_ptr(), max(out.stride(0), H * hd), B, H, float(scale), int(window), int(sinks), int(max_len),
-                   self._workspace.data_ptr(), self._workspace.numel())
+            ld = H * hd
+        else:
+            if out.shape != (B, H * hd) or out.dtype != torch.float16 or (out.stride(1) != 1 and out.numel() > 0):
+                raise ValueError(f"out must be fp16 {(B, H * hd)} with a contiguous last dimension")
+            tk.require_cuda(self.pages, out)
+            ld = out.stride(0) if B > 1 else H * hd
+        if slots is not None:
+            slots = self._slots(slots)
+            if slots.numel() != B:
+                raise ValueError(f"{B} rows, but {slots.numel()} slots")
+        self._call("tk_attn_decode", int(layer), q.data_ptr(), qs[0], qs[1], *new, tk.ptr(slots), out.data_ptr(), ld,
+                   B, H, float(scale), int(window), int(sinks), int(max_len), self._workspace_ptr,
+                   self._workspace_bytes)
         return out
 
     # -- helpers ---------------------------------------------------------------------
     def _call(self, name: str, *args) -> None:
-        with torch.cuda.device(self.device):
-            tk.call(name, ctypes.byref(self._c), *args, tk.stream_handle(self.device))
+        tk.call_on(self.device, name, self._handle, *args)
 
     def _check_data(self, what: str, *tensors: torch.Tensor) -> None:
-        tk.require_cuda(self.pages, *tensors)
         for t in tensors:
+            if t.device != self.device:
+                tk.require_cuda(self.pages, *tensors)
             if t.dtype != torch.float16:
                 raise tk.TKError(what, -2, "the cache and its inputs are float16")
-            if t.numel() and t.stride(-1) != 1:
+            if t.stride(-1) != 1 and t.numel():
                 raise tk.TKError(what, -1, "inputs need a contiguous last dimension")
-        if len(tensors) == 2 and _strides(tensors[0]) != _strides(tensors[1]):
+        if len(tensors) == 2 and tensors[0].stride() != tensors[1].stride() \
+                and _strides(tensors[0]) != _strides(tensors[1]):
             raise tk.TKError(what, -1, "keys and values need identical strides")
 
     def _upload(self, values: Sequence[int]) -> torch.Tensor:
@@ -297,7 +308,8 @@ class PagedCache:
             return self._upload([int(x) for x in values])
         if values.dim() != 1 or values.dtype != torch.int32:
             raise ValueError(f"{name} must be a one-dimensional int32 tensor or a list of ints")
-        tk.require_cuda(self.pages, values)
+        if values.device != self.device:
+            tk.require_cuda(self.pages, values)
         return values.contiguous()
 
     def _slots(self, slots: Slots) -> torch.Tensor:
