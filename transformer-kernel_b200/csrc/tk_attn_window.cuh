@@ -137,6 +137,24 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
   }
 }
 
+// Shared-memory matrix descriptor whose start moves by constants: only its low
+// word changes (addresses stay below 2^18, so the 14-bit field never carries).
+// One thread issues every product, and what it executes between two of them
+// adds up: rebuilding both descriptors each time and splitting P V into 64
+// columns made the issuer the slowest role at hd 128.
+struct Desc {
+  uint32_t lo, hi;
+
+  __device__ __forceinline__ Desc(uint32_t addr, uint32_t lbo, uint32_t sbo, SmemLayout layout) {
+    const uint64_t d = smem_desc(addr, lbo, sbo, layout);
+    lo = static_cast<uint32_t>(d);
+    hi = static_cast<uint32_t>(d >> 32);
+  }
+  __device__ __forceinline__ uint64_t at(int bytes) const {
+    return (static_cast<uint64_t>(hi) << 32) | (lo + static_cast<uint32_t>(bytes >> 4));
+  }
+};
+
 // The lowest n bits of a word (n clamped to 0..32).
 __device__ __forceinline__ uint32_t low_bits(int n) {
   return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
@@ -267,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---------------- MMA issuer ----------------
       if (lane == 0) {
         constexpr uint32_t idesc_s = idesc_f16_f32(kBM, kBN, false, false);
-        constexpr uint32_t idesc_o = idesc_f16_f32(kBM, C::COLS, false, true);
+        constexpr uint32_t idesc_o = idesc_f16_f32(kBM, HD, false, true);
         struct Group {
           int tiles = 0;     // products P V issued (p_full, pv_done phases)
           int o_uses = 0;    // items in which O_g was accumulated (o_full / o_free phases)
@@ -316,16 +334,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             ++gs.s_issued;
             tc_fence_after();
-            const uint32_t q_addr = smem_u32(sQ + (qs * C::GROUPS + g) * C::TILE_BYTES);
-            const uint32_t k_addr = smem_u32(sR + ((base + 2 * j) % SLOTS) * C::TILE_BYTES);
-#pragma unroll 1
-            for (int c = 0; c < C::NC; ++c)
-#pragma unroll
-              for (int kk = 0; kk < C::COLS / 16; ++kk) {
-                const uint64_t dq = smem_desc(q_addr + c * C::CHUNK_BYTES + kk * 32, 16, C::SBO, C::LAYOUT);
-                const uint64_t dk = smem_desc(k_addr + c * C::CHUNK_BYTES + kk * 32, 16, C::SBO, C::LAYOUT);
-                mma_f16_ss(tmem_base + C::col_s(g), dq, dk, idesc_s, (c | kk) != 0 ? 1u : 0u);
-              }
+            const Desc dq(smem_u32(sQ + (qs * C::GROUPS + g) * C::TILE_BYTES), 16, C::SBO, C::LAYOUT);
+            const Desc dk(smem_u32(sR + ((base + 2 * j) % SLOTS) * C::TILE_BYTES), 16, C::SBO, C::LAYOUT);
+#pragma unroll(HD == 256 ? 4 : HD / 16)
+            for (int kk = 0; kk < HD / 16; ++kk) {
+              const int at = kk / (C::COLS / 16) * C::CHUNK_BYTES + kk % (C::COLS / 16) * 32;
+              mma_f16_ss(tmem_base + C::col_s(g), dq.at(at), dk.at(at), idesc_s, kk != 0 ? 1u : 0u);
+            }
             mma_commit(&s_full[g]);
             if (last_reader) mma_commit(&slot_empty[(base + 2 * j) % SLOTS]);
           };
@@ -344,16 +359,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               return;
             }
             tc_fence_after();
-            const uint32_t v_addr = smem_u32(sR + ((base + 2 * j + 1) % SLOTS) * C::TILE_BYTES);
-#pragma unroll 1
-            for (int c = 0; c < C::NC; ++c)
+            // V is MN-major: 8 keys x COLS columns a swizzle atom, CHUNK_BYTES to
+            // the next COLS columns, so one product spans the whole head
+            const Desc dv(smem_u32(sR + ((base + 2 * j + 1) % SLOTS) * C::TILE_BYTES), C::CHUNK_BYTES, C::SBO,
+                          C::LAYOUT);
 #pragma unroll
-              for (int ks = 0; ks < kBN / 16; ++ks) {
-                const uint64_t dv = smem_desc(v_addr + c * C::CHUNK_BYTES + ks * 16 * C::ROW_BYTES, C::CHUNK_BYTES,
-                                              C::SBO, C::LAYOUT);
-                mma_f16_ts(tmem_base + C::col_o(g) + c * C::COLS, tmem_base + C::col_p(g) + ks * 8, dv, idesc_o,
-                           (gs.in_item > 0 || ks > 0) ? 1u : 0u);
-              }
+            for (int ks = 0; ks < kBN / 16; ++ks)
+              mma_f16_ts(tmem_base + C::col_o(g), tmem_base + C::col_p(g) + ks * 8, dv.at(ks * 16 * C::ROW_BYTES),
+                         idesc_o, (gs.in_item > 0 || ks > 0) ? 1u : 0u);
             mma_commit(&pv_done[g]);
             if (last_reader) mma_commit(&slot_empty[(base + 2 * j + 1) % SLOTS]);
             if (++gs.in_item == n_g) {
