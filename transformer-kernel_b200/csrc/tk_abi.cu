@@ -907,7 +907,9 @@ int launch_window(DeviceInfo* info, int slot, const CUtensorMap (&maps)[3], cons
     }
   }
   const int64_t q_tiles = (p.S + 127) / 128;
-  const int64_t items = static_cast<int64_t>(p.B) * p.H * ((q_tiles + C::GROUPS - 1) / C::GROUPS);
+  const int64_t heads = static_cast<int64_t>(p.B) * p.H;
+  const int64_t items = C::GROUPS == 2 && p.pair_heads ? heads / 2 * q_tiles
+                                                       : heads * ((q_tiles + C::GROUPS - 1) / C::GROUPS);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(items, info->sms));
   return launched(launch(kern, dim3(grid), dim3(tk::attn::kThreads), C::SMEM_BYTES, s, small, maps[0], maps[1],
                          maps[2], p),
@@ -961,6 +963,7 @@ int tk_attn_window(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_
   p.S = static_cast<int>(S);
   p.H = static_cast<int>(H);
   p.G = static_cast<int>(H / Hkv);
+  p.pair_heads = p.G % 2 == 0;
   p.window = static_cast<int>(std::min(window, S));
   p.sinks = static_cast<int>(std::min(sinks, S));
   p.scale_log2 = scale * 1.4426950408889634f;

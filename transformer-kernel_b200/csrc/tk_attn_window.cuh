@@ -48,6 +48,7 @@ struct Params {
   int64_t ld_out;
   int B, S, H, G;       // G = H / Hkv
   int window, sinks;    // window >= 1
+  int pair_heads;       // the groups of an item take two heads of one tile (G even), else two tiles of one head
   float scale_log2;
   const int* kv_len;    // optional [B]
   int q_heads_inner, kv_heads_inner;  // tensor-map dim order, as attn::Params
@@ -80,11 +81,14 @@ struct Cfg {
 enum : unsigned { kSiteQ = 1, kSiteSlot = 2, kSiteS = 3, kSiteP = 4, kSiteO = 5, kSiteEmpty = 6, kSiteOFree = 7,
                   kSiteQEmpty = 8, kSitePv = 9, kSiteSFree = 10, kSiteClean = 11 };
 
-// One work item: head h of sequence b, query tiles tq0 and (has1) tq0 + 1.
+// One work item: group 0 takes head h of sequence b and query tile tq0, group 1
+// (has1) head h + dh and tile tq0 + dq, one of them 0 and the other 1. Two heads
+// of one key-value head need the same key tiles; two tiles of one head need one
+// tile more than either.
 // Step j works on key tile tile(j); group 0 takes steps j < n0, group 1 all
 // but `skip`.
 struct Item {
-  int b, h, tq0, kv_bound;
+  int b, h, tq0, dh, dq, kv_bound;
   int n_sink, lo;       // steps of the first tokens' tiles; first window tile
   int n, n0, n1, skip;
   int dirty;            // step whose value tile reaches past kv_len (-1: none)
@@ -97,19 +101,23 @@ struct Item {
 template <int GROUPS>
 __device__ __forceinline__ Item make_item(const Params& p, int idx, int q_tiles, int q_items) {
   Item it;
-  const int bh_count = p.B * p.H;
+  const bool pair = GROUPS == 2 && p.pair_heads;
+  it.dh = pair ? 1 : 0;
+  it.dq = 1 - it.dh;
+  const int heads = p.H >> it.dh, bh_count = p.B * heads;
   const int bh = idx % bh_count;
-  it.b = bh / p.H;
-  it.h = bh % p.H;
-  it.tq0 = GROUPS * (q_items - 1 - idx / bh_count);  // full windows first, the first rows' short ones last
-  it.has1 = GROUPS == 2 && it.tq0 + 1 < q_tiles;
+  it.b = bh / heads;
+  it.h = (bh % heads) << it.dh;
+  // full windows first, the first rows' short ones last
+  it.tq0 = (pair ? 1 : GROUPS) * (q_items - 1 - idx / bh_count);
+  it.has1 = pair || (GROUPS == 2 && it.tq0 + 1 < q_tiles);
   it.kv_bound = p.S;
   if (p.kv_len != nullptr) it.kv_bound = max(0, min(p.S, p.kv_len[it.b]));
   const int n_kv = (it.kv_bound + kBN - 1) / kBN;
   const int sink_tiles = (min(p.sinks, it.kv_bound) + kBN - 1) / kBN;
   it.lo = max(0, it.tq0 * kBM - p.window + 1) / kBN;
-  const int lo1 = max(0, (it.tq0 + 1) * kBM - p.window + 1) / kBN;
-  const int hi0 = min(it.tq0, n_kv - 1), hi1 = it.has1 ? min(it.tq0 + 1, n_kv - 1) : hi0;
+  const int lo1 = max(0, (it.tq0 + it.dq) * kBM - p.window + 1) / kBN;
+  const int hi0 = min(it.tq0, n_kv - 1), hi1 = it.has1 ? min(it.tq0 + it.dq, n_kv - 1) : hi0;
   it.n_sink = min(sink_tiles, it.lo);
   it.n = it.n_sink + max(0, hi1 - it.lo + 1);
   it.n0 = it.n - (hi1 - hi0);
@@ -190,8 +198,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = warp_id_uniform();
   const uint32_t lane = lane_id();
   const int q_tiles = (p.S + kBM - 1) / kBM;
-  const int q_items = (q_tiles + C::GROUPS - 1) / C::GROUPS;
-  const int n_items = q_items * p.B * p.H;
+  const bool pair = C::GROUPS == 2 && p.pair_heads;
+  const int q_items = pair ? q_tiles : (q_tiles + C::GROUPS - 1) / C::GROUPS;
+  const int n_items = q_items * p.B * (pair ? p.H / 2 : p.H);
   const unsigned kid = 0xC0u + HD / 16;
 
   if (threadIdx.x == 0) {
@@ -254,8 +263,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_expect_tx(&q_full[qs], C::TILE_BYTES * (it.has1 ? 2 : 1));
           load_tile<HD>(q_dst, &map_q, &q_full[qs], p.q_heads_inner, it.tq0 * kBM, it.h, it.b);
           if (it.has1)
-            load_tile<HD>(q_dst + C::TILE_BYTES, &map_q, &q_full[qs], p.q_heads_inner, (it.tq0 + 1) * kBM, it.h,
-                          it.b);
+            load_tile<HD>(q_dst + C::TILE_BYTES, &map_q, &q_full[qs], p.q_heads_inner, (it.tq0 + it.dq) * kBM,
+                          it.h + it.dh, it.b);
           const int kvh = it.h / p.G;
           for (int j = 0; j < 2 * it.n; ++j, ++n) {
             const int s = n % SLOTS;
@@ -468,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item it = make_item<C::GROUPS>(p, idx, q_tiles, q_items);
       if (g == 1 && !it.has1) continue;
       const int n_g = g == 0 ? it.n0 : it.n1;
-      const int q_idx = (it.tq0 + g) * kBM + r;
+      const int q_idx = (it.tq0 + g * it.dq) * kBM + r;
       float m = -INFINITY;  // running max, raw score units
       float l = 0.f;
       int done = 0;         // steps of this item so far
@@ -616,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // a row that sees no key has m = -inf: zeros
       const float inv_l = (m != -INFINITY) ? 1.f / l : 0.f;
-      __half* dst = p.out + (static_cast<int64_t>(it.b) * p.S + q_idx) * p.ld_out + it.h * p.hd;
+      __half* dst = p.out + (static_cast<int64_t>(it.b) * p.S + q_idx) * p.ld_out + (it.h + g * it.dh) * p.hd;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 16) {
         uint32_t o[16];
