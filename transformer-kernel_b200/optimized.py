@@ -28,6 +28,12 @@ Forward, per layer (``T = B*S`` token rows, fp32 residual stream):
 
 The final LayerNorm writes the fp32 output directly. There is no CPU,
 SDPA, cuBLAS or Triton path: anything the kernels cannot do raises.
+
+A causal model also serves: ``prefill`` runs prompts like ``forward`` and keeps
+every layer's keys and values in a ``paged_cache.PagedCache``, ``decode_step``
+adds one token to each sequence and attends over the cache, both with an
+optional sliding window. The reference recomputes the whole sequence for every
+new token (:488-554).
 """
 
 from __future__ import annotations
@@ -42,6 +48,7 @@ import torch.nn as nn
 import _tklib as tk
 import kernels
 import linear as tk_linear
+from paged_cache import PagedCache, Slots
 
 __all__ = ["OptimizerSettings", "OptimizedTransformer", "TransformerConfig", "configure", "active_settings"]
 
@@ -376,10 +383,11 @@ class OptimizedTransformer(nn.Module):
         self._launch("ln_in", self._layer_norm, xin, w0.norm1_w, w0.norm1_b, w0.norm1_eps, h, copy_to=res)
 
     def _body(self, B: int, S: int, lengths: Optional[torch.Tensor], bufs, weights: List[_LayerWeights],
-              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+              out: Optional[torch.Tensor] = None, attend=None) -> torch.Tensor:
         """Every launch after ``_head``: the layers (the residual stream is
         updated in place) and the final LayerNorm into ``out`` (default the
-        forward's own output buffer). Returns the output as [B, S, d]."""
+        forward's own output buffer). Returns the output as [B, S, d].
+        ``attend(layer, q, k, v, ctx)`` replaces the attention launch."""
         res, h, qkv, ctx, u, out_ws, ln_ws = bufs
         T, d = res.shape
         ffn = u.shape[1]
@@ -395,8 +403,11 @@ class OptimizedTransformer(nn.Module):
         last = len(weights) - 1
         for i, w in enumerate(weights):
             run("gemm_qkv", lin, h, w.qkv_w, w.qkv_b, "bias", out=qkv)
-            run("attn", kernels.flash_attention, q, k, v, self.attn_scale, self.config.causal,
-                kv_len=lengths, out=ctx)
+            if attend is None:
+                run("attn", kernels.flash_attention, q, k, v, self.attn_scale, self.config.causal,
+                    kv_len=lengths, out=ctx)
+            else:
+                attend(i, q, k, v, ctx)
             ctx2 = ctx.view(T, d)
             if fused:
                 run("gemm_o_ln", lin, ctx2, w.out_w, w.out_b, "resid_ln", resid=res, sum_out=res,
@@ -430,6 +441,93 @@ class OptimizedTransformer(nn.Module):
             bufs = self._activations(B, S, d, weights[0].ffn_in_w.shape[0], dev)
             self._head(x, bufs, weights)
             return self._body(B, S, lengths, bufs, weights, out)
+
+    # -- serving ------------------------------------------------------------------
+    def _check_cache(self, cache: PagedCache, device: torch.device, window: int, sinks: int) -> None:
+        if not self.config.causal:
+            raise tk.TKError("serving", -2, "only a causal model can keep its keys and values while it generates")
+        want = (len(self.layers), self.num_heads, self.head_dim)
+        if (cache.num_layers, cache.kv_heads, cache.head_dim) != want:
+            raise ValueError(f"the model has (layers, heads, head_dim) = {want}, the cache "
+                             f"{(cache.num_layers, cache.kv_heads, cache.head_dim)}")
+        if cache.device != device:
+            raise tk.TKError("device", -1, f"tensors on different devices: {device} vs {cache.device}")
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks cannot be negative")
+
+    @_outside_compile
+    def prefill(
+        self,
+        x: torch.Tensor,
+        cache: PagedCache,
+        slots: Slots,
+        valid_token_mask: Optional[torch.Tensor] = None,
+        window: int = 0,
+        sinks: int = 0,
+    ) -> torch.Tensor:
+        """``forward`` over prompts, which also fills the empty ``slots`` of
+        the cache (row b's valid tokens go to ``slots[b]``). With ``window`` >
+        0 a token sees the ``window`` latest keys and the first ``sinks``
+        ones. Returns ``[B, S, d]`` in x's dtype."""
+        self._check_input(x)
+        self._check_cache(cache, x.device, window, sinks)
+        B, S, d = x.shape
+        if B * S == 0:
+            raise ValueError(f"prompts need at least one row and one token, got {tuple(x.shape)}")
+        lengths = self._prefix_lengths(valid_token_mask)
+        counts = torch.full((B,), S, dtype=torch.int32, device=x.device) if lengths is None else lengths
+        slots = cache._slots(slots)
+        cache.reserve(slots, counts, require_empty=True)
+
+        def attend(layer, q, k, v, ctx):
+            self._launch("kv_store", cache.store, layer, k, v, slots, counts)
+            if window > 0:
+                self._launch("attn", kernels.window_attention, q, k, v, self.attn_scale, window, sinks,
+                             kv_len=lengths, out=ctx)
+            else:
+                self._launch("attn", kernels.flash_attention, q, k, v, self.attn_scale, True, kv_len=lengths, out=ctx)
+
+        weights = self._weights()
+        with torch.cuda.device(x.device):
+            bufs = self._activations(B, S, d, weights[0].ffn_in_w.shape[0], x.device)
+            self._head(x, bufs, weights)
+            return self._finish(x, self._body(B, S, lengths, bufs, weights, attend=attend))
+
+    @_outside_compile
+    def decode_step(
+        self,
+        x: torch.Tensor,
+        cache: PagedCache,
+        slots: Slots,
+        window: int = 0,
+        sinks: int = 0,
+        max_len: int = 0,
+    ) -> torch.Tensor:
+        """One more token for each sequence: ``x`` ``[B, d]`` is appended to
+        ``slots`` and attends over what the cache holds. Returns ``[B, d]`` in
+        x's dtype; rows with slot -1 are padding and hold nothing of use. Can
+        be captured into a CUDA graph (with ``slots`` a tensor). ``max_len``:
+        as for ``PagedCache.attend``."""
+        if x.dim() != 2 or x.shape[1] != self.d_model:
+            raise ValueError(f"expected x of shape [B, {self.d_model}], got {tuple(x.shape)}")
+        self._check_input(x[:, None])
+        self._check_cache(cache, x.device, window, sinks)
+        B, d = x.shape
+        if B == 0:
+            return x.clone()
+        slots = cache._slots(slots)
+        cache.reserve(slots, torch.ones(B, dtype=torch.int32, device=x.device))
+
+        def attend(layer, q, k, v, ctx):
+            self._launch("attn_decode", cache.attend, layer, q[:, :, 0], self.attn_scale, k_new=k[:, :, 0],
+                         v_new=v[:, :, 0], slots=slots, window=window, sinks=sinks, max_len=max_len,
+                         out=ctx.view(B, d))
+
+        weights = self._weights()
+        with torch.cuda.device(x.device):
+            bufs = self._activations(B, 1, d, weights[0].ffn_in_w.shape[0], x.device)
+            self._head(x[:, None], bufs, weights)
+            return self._finish(x, self._body(B, 1, None, bufs, weights, attend=attend).view(B, d))
 
     # -- host-streamed forward --------------------------------------------------
     @_outside_compile
