@@ -106,22 +106,30 @@ def window_attention(
         raise ValueError(f"sizes must be positive and {H} query heads a multiple of {Hkv} key-value heads")
     if not (q.dtype == k.dtype == v.dtype == torch.float16):
         raise tk.TKError("window_attention", -2, "q/k/v must be float16")
-    qs, ks = q.stride(), k.stride()
-    if ks != v.stride() or qs[3] != 1 or ks[3] != 1:
+    q_b, q_h, q_s, q_1 = q.stride()
+    k_b, k_h, k_s, k_1 = strides = k.stride()
+    if strides != v.stride() or q_1 != 1 or k_1 != 1:
         raise tk.TKError("window_attention", -1, "k and v need identical strides, and all a contiguous last dimension")
-    dev = tk.require_cuda(q, k, v, kv_len, out)
+    dev = q.device
+    if dev.type != "cuda" or k.device != dev or v.device != dev:
+        tk.require_cuda(q, k, v)
+    ld = H * hd
     if out is None:
-        out = torch.empty((B, S, H * hd), dtype=torch.float16, device=dev)
-        ld = H * hd
+        out = q.new_empty((B, S, ld))
     else:
-        ld = out.stride(1) if S > 1 else max(out.stride(1), H * hd)
+        tk.require_cuda(q, out)
+        if S > 1 or out.stride(1) > ld:
+            ld = out.stride(1)
         if (out.shape != (B, S, H * hd) or out.dtype != torch.float16 or out.stride(2) != 1
                 or (B > 1 and out.stride(0) != S * ld)):
             raise ValueError("out must be fp16 [B, S, H*hd] with unit last stride and rows S*ld apart per batch")
+    kv_ptr = None
     if kv_len is not None:
+        tk.require_cuda(q, kv_len)
         if kv_len.shape != (B,):
             raise ValueError(f"kv_len must have shape ({B},), got {tuple(kv_len.shape)}")
         kv_len = kv_len.to(dtype=torch.int32).contiguous()
-    tk.call_on(dev, "tk_attn_window", q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), v.data_ptr(), ks[0], ks[1],
-               ks[2], out.data_ptr(), ld, B, S, H, Hkv, hd, float(scale), int(window), int(sinks), tk.ptr(kv_len))
+        kv_ptr = kv_len.data_ptr()
+    tk.call_on(dev, "tk_attn_window", q.data_ptr(), q_b, q_h, q_s, k.data_ptr(), v.data_ptr(), k_b, k_h, k_s,
+               out.data_ptr(), ld, B, S, H, Hkv, hd, scale, window, sinks, kv_ptr)
     return out

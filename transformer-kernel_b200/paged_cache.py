@@ -123,7 +123,7 @@ class PagedCache:
             page_table.data_ptr(), self.seq_lens.data_ptr(), self.ref_counts.data_ptr(), mask.data_ptr(),
             status.data_ptr(), live.data_ptr(), self._scratch.data_ptr(), pages.data_ptr(), max_seqs,
             max_pages_per_seq, num_pages, page_size, num_layers, kv_heads, head_dim)
-        self._handle = ctypes.byref(self._c)
+        self._handle, self._lib, self._index = ctypes.byref(self._c), tk.lib(), self.device.index
         self._workspace_ptr, self._workspace_bytes = self._workspace.data_ptr(), need
         self.reset()
 
@@ -255,38 +255,51 @@ class PagedCache:
         if len(shape) != 3 or shape[2] != hd or shape[1] == 0 or shape[1] % K:
             raise ValueError(f"q must be [B, a multiple of {K} heads, {hd}], got {tuple(shape)}")
         B, H, _ = shape
-        self._check_data("attend", q)
-        qs = q.stride()
-        new = (None, None, 0, 0)
-        if k_new is not None and v_new is not None:
+        q_b, q_h, q_1 = q.stride()
+        if q.dtype != torch.float16 or q.device != self.device or q_1 != 1:
+            self._check_data("attend", q)
+        if k_new is None and v_new is None:
+            k_ptr, v_ptr, k_b, k_h = None, None, 0, 0
+        elif k_new is None or v_new is None:
+            raise ValueError("k_new and v_new come together")
+        else:
             if not (k_new.shape == v_new.shape == (B, K, hd)):
                 raise ValueError(f"k_new/v_new must be {(B, K, hd)}, got {tuple(k_new.shape)} and "
                                  f"{tuple(v_new.shape)}")
-            self._check_data("attend", k_new, v_new)
-            ns = k_new.stride()
-            new = (k_new.data_ptr(), v_new.data_ptr(), ns[0], ns[1])
-        elif k_new is not None or v_new is not None:
-            raise ValueError("k_new and v_new come together")
+            k_b, k_h, k_1 = strides = k_new.stride()
+            if (not (k_new.dtype == v_new.dtype == torch.float16) or not (k_new.device == v_new.device == self.device)
+                    or k_1 != 1 or v_new.stride() != strides):
+                self._check_data("attend", k_new, v_new)
+            k_ptr, v_ptr = k_new.data_ptr(), v_new.data_ptr()
+        ld = H * hd
         if out is None:
-            out = torch.empty((B, H * hd), dtype=torch.float16, device=self.device)
-            ld = H * hd
+            out = q.new_empty((B, ld))
         else:
-            if out.shape != (B, H * hd) or out.dtype != torch.float16 or (out.stride(1) != 1 and out.numel() > 0):
-                raise ValueError(f"out must be fp16 {(B, H * hd)} with a contiguous last dimension")
-            tk.require_cuda(self.pages, out)
-            ld = out.stride(0) if B > 1 else H * hd
+            if out.shape != (B, ld) or out.dtype != torch.float16 or (out.stride(1) != 1 and out.numel() > 0):
+                raise ValueError(f"out must be fp16 {(B, ld)} with a contiguous last dimension")
+            if out.device != self.device:
+                tk.require_cuda(self.pages, out)
+            if B > 1:
+                ld = out.stride(0)
+        slots_ptr = None
         if slots is not None:
             slots = self._slots(slots)
             if slots.numel() != B:
                 raise ValueError(f"{B} rows, but {slots.numel()} slots")
-        self._call("tk_attn_decode", int(layer), q.data_ptr(), qs[0], qs[1], *new, tk.ptr(slots), out.data_ptr(), ld,
-                   B, H, float(scale), int(window), int(sinks), int(max_len), self._workspace_ptr,
-                   self._workspace_bytes)
+            slots_ptr = slots.data_ptr()
+        self._call("tk_attn_decode", layer, q.data_ptr(), q_b, q_h, k_ptr, v_ptr, k_b, k_h, slots_ptr, out.data_ptr(),
+                   ld, B, H, scale, window, sinks, max_len, self._workspace_ptr, self._workspace_bytes)
         return out
 
     # -- helpers ---------------------------------------------------------------------
     def _call(self, name: str, *args) -> None:
-        tk.call_on(self.device, name, self._handle, *args)
+        index = self._index
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
+                return self._call(name, *args)
+        status = getattr(self._lib, name)(self._handle, *args, tk.stream_handle(self.device))
+        if status != tk.TK_OK:
+            raise tk.TKError(name, status, self._lib.tk_last_error().decode(errors="replace"))
 
     def _check_data(self, what: str, *tensors: torch.Tensor) -> None:
         for t in tensors:
