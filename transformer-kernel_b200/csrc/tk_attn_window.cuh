@@ -533,29 +533,42 @@ __global__ void __launch_bounds__(kThreads, 1)
         // a masked score is -inf and gives 0 (the FMA-pipe exponential clamps
         // it at 2^-126, which the fp16 P rounds to 0)
         const float neg_mc = (m_use == -INFINITY) ? 0.f : -m_use * sl;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int t = 0; t < 32; t += 2) {
-            float x0, x1;
-            fma2(x0, x1, __uint_as_float(sv[c][t]), __uint_as_float(sv[c][t + 1]), sl, neg_mc);
-            sv[c][t] = __float_as_uint(x0);
-            sv[c][t + 1] = __float_as_uint(x1);
-          }
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int t = 0; t < 32; t += 2) exp2_cols(sv[c][t], sv[c][t + 1], t);
+        // Eight columns at a time, one group's exponentials between the next
+        // one's scaling and the previous one's sums and packing: the SFU takes
+        // a warp's exponential every 8 clocks, which leaves issue slots for
+        // the other two.
         float rs[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        auto pack = [&](int c, uint32_t (&pk)[16]) {
+        uint32_t pk[4][16];
+        auto scale8 = [&](int u) {
 #pragma unroll
-          for (int t = 0; t < 32; t += 2) {
-            const float p0 = __uint_as_float(sv[c][t]), p1 = __uint_as_float(sv[c][t + 1]);
-            const int a = ((t >> 1) & 3) * 2;
-            add2(rs[a], rs[a + 1], p0, p1);
-            pk[t / 2] = pack_half2(p0, p1);
+          for (int t = (u & 3) * 8; t < (u & 3) * 8 + 8; t += 2) {
+            float x0, x1;
+            fma2(x0, x1, __uint_as_float(sv[u >> 2][t]), __uint_as_float(sv[u >> 2][t + 1]), sl, neg_mc);
+            sv[u >> 2][t] = __float_as_uint(x0);
+            sv[u >> 2][t + 1] = __float_as_uint(x1);
           }
         };
+        auto exp8 = [&](int u) {
+#pragma unroll
+          for (int t = (u & 3) * 8; t < (u & 3) * 8 + 8; t += 2) exp2_cols(sv[u >> 2][t], sv[u >> 2][t + 1], t);
+        };
+        auto pack8 = [&](int u) {
+#pragma unroll
+          for (int t = (u & 3) * 8; t < (u & 3) * 8 + 8; t += 2) {
+            const float p0 = __uint_as_float(sv[u >> 2][t]), p1 = __uint_as_float(sv[u >> 2][t + 1]);
+            const int a = ((t >> 1) & 3) * 2;
+            add2(rs[a], rs[a + 1], p0, p1);
+            pk[u >> 2][t / 2] = pack_half2(p0, p1);
+          }
+        };
+        scale8(0);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          if (u < 15) scale8(u + 1);
+          exp8(u);
+          if (u > 0) pack8(u - 1);
+        }
+        pack8(15);
         // The previous step's product reads P_g and writes O_g: complete before
         // P_g is overwritten or O_g rescaled. (Where P_g lies over S_g, this
         // step's scores were only issued after it.)
@@ -569,27 +582,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           return true;
         };
-        if constexpr (HD <= 64) {
-          // packed during the previous product
-          uint32_t pk[4][16];
+        ok = wait_pv();
+        if (!ok) break;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) pack(c, pk[c]);
-          ok = wait_pv();
-          if (!ok) break;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_st16(t_p + c * 16, pk[c]);
-        } else {
-          // a quarter at a time: with the packed row beside the scores these
-          // kernels spill
-          ok = wait_pv();
-          if (!ok) break;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
-            pack(c, pk);
-            tmem_st16(t_p + c * 16, pk);
-          }
-        }
+        for (int c = 0; c < 4; ++c) tmem_st16(t_p + c * 16, pk[c]);
         const float row_sum = ((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]));
         const bool need = (done > 0) && (alpha != 1.f);
         if (__any_sync(0xffffffffu, need)) {
