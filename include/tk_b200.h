@@ -262,12 +262,14 @@ TK_API int tk_copy_rows(void* dst, int64_t dst_ld, const void* src, int64_t src_
  * page_size is a power of two in 16..256; max_seqs <= 8192, table_width and
  * num_pages <= 2^20. Pages are taken lowest first in the order of the call's
  * entries, so the state that a call leaves depends on its arguments and the
- * books alone. A call on a cache applies whole or not at all: when an entry
- * is refused nothing changes, the status word and the device error word are
- * set, and until the caller zeroes the status word later calls on the cache
- * do nothing. Slot lists are int32 on the device, at most 8192 entries, each
- * slot at most once; slot -1 is padding. Calls on one cache must be ordered
- * on the GPU. */
+ * books alone. A call applies whole or not at all: when an entry is refused
+ * nothing changes, the status word and the device error word are set, and
+ * until the caller zeroes the status word later calls on the cache do nothing
+ * (tk_attn_decode then leaves its output as it is). tk_attn_decode reports a
+ * slot or a length that cannot be the same way; that call's output is then
+ * unspecified. Slot lists are int32 on the device, at most 8192 entries, each
+ * slot at most once; slot -1 is padding. Calls on one cache must be ordered on
+ * the GPU. */
 typedef struct tk_cache {
   int32_t* page_table;
   int32_t* seq_lens;

@@ -383,6 +383,49 @@ def test_wrong_arguments_raise(cuda_device):
     cache.check()
 
 
+@gpu
+def test_alignment_is_checked(cuda_device):
+    """Rows that 16-byte loads cannot take are refused before a launch; a
+    dimension of one entry may have any stride."""
+    cache, _ = make()
+    cache.reserve([0, 1], [4, 4])
+    flat = torch.zeros(4096, device="cuda").half()
+    q = flat[:256].view(2, 4, 32)
+    off = flat[4:4 + 2 * 2 * 32].view(2, 2, 32)                      # 8 bytes off
+    odd = torch.as_strided(flat, (2, 2, 32), (100, 36, 1))           # rows 72 bytes apart
+    for k in (off, odd):
+        with pytest.raises(tk.TKError, match="16-byte"):
+            cache.attend(0, q, 1.0, k_new=k, v_new=k)
+    with pytest.raises(tk.TKError, match="even strides"):
+        cache.attend(0, torch.as_strided(flat, (2, 4, 32), (129, 32, 1)), 1.0)
+    with pytest.raises(tk.TKError, match="4-byte aligned rows"):
+        cache.attend(0, q, 1.0, out=torch.as_strided(flat, (2, 128), (131, 1)))
+    with pytest.raises(tk.TKError, match="16-byte"):
+        kv = torch.as_strided(flat, (2, 2, 4, 32), (1001, 128, 32, 1))
+        cache.store(0, kv, kv, [0, 1])
+    one = torch.as_strided(flat, (1, 2, 32), (7, 32, 1))
+    cache.attend(0, torch.as_strided(flat, (1, 4, 32), (3, 32, 1)), 1.0, k_new=one, v_new=one, slots=[1])
+    token = torch.as_strided(flat, (1, 2, 1, 32), (5, 32, 3, 1))
+    cache.store(0, token, token, [0])
+    cache.check()
+    tk.check_device_errors(cuda_device)
+
+
+@gpu
+@pytest.mark.parametrize("slots, bit", [((0, 5, 1), 4), ((0, 1, 1), 2), ((0, 1, 8), 2)])
+def test_store_applies_whole_or_not_at_all(cuda_device, slots, bit):
+    """One row that cannot be (an empty slot, a slot twice, a slot that does
+    not exist): the other rows are not stored either."""
+    cache, _ = make(layers=1, kv_heads=1, head_dim=16)
+    cache.pages.zero_()
+    cache.reserve([0, 1], [4, 4])
+    k = torch.ones(3, 1, 4, 16, device="cuda").half()
+    cache.store(0, k, k, ints(*slots))
+    assert int(cache.status) == bit and not cache.pages.any()
+    with pytest.raises(tk.TKError):
+        tk.check_device_errors(cuda_device)
+
+
 # ---------------------------------------------------------------------------
 # decode attention
 # ---------------------------------------------------------------------------
@@ -619,6 +662,29 @@ def test_decode_reports_bad_books(cuda_device):
     cache, kv, g = filled([40, 20], 16, 2, 64)
     cache.attend(0, q, 0.1, slots=ints(0, 5))
     assert int(cache.status) == 2
+    with pytest.raises(tk.TKError):
+        tk.check_device_errors(cuda_device)
+
+
+@gpu
+@pytest.mark.parametrize("rows, kv_heads, width", [(2, 2, 3), (40, 16, 3), (5, 2, 400)])
+def test_decode_refuses_two_new_tokens_for_one_sequence(cuda_device, rows, kv_heads, width):
+    """In every division of the work (a CTA or a warp per segment, split);
+    without new tokens a sequence may be read by several rows."""
+    cache, kv, g = filled([40] * rows, 16, kv_heads, 64, width=width)
+    before = cache.pages.clone()
+    q = torch.randn(rows, kv_heads, 64, generator=g, device="cuda").half()
+    slots = torch.arange(rows, dtype=torch.int32, device="cuda")
+    slots[rows - 1] = 0
+    out = cache.attend(0, q, 0.125, slots=slots)
+    for b, s in ((0, 0), (rows - 1, 0)):
+        ref, tol = attend_reference(q[b], kv[s][0], kv[s][1], 0.125)
+        assert bool(((out[b].view(kv_heads, 64).double() - ref).abs() <= tol).all())
+    cache.check()
+    cache.attend(0, q, 0.125, k_new=q, v_new=q, slots=slots)
+    assert int(cache.status) == 2
+    page = cache.page_table[0, 2].long()
+    assert torch.equal(cache.pages[0, page].view(torch.int16), before[0, page].view(torch.int16))
     with pytest.raises(tk.TKError):
         tk.check_device_errors(cuda_device)
 

@@ -1253,7 +1253,7 @@ int tk_cache_store(const tk_cache* cache, int64_t layer, const void* k, const vo
   const int64_t vecs = S * p.heads * p.row_vecs;
   const int64_t blocks = std::min<int64_t>((vecs + 255) / 256, std::max<int64_t>(1, 16ll * info->sms / B));
   return launched(launch(tk::paged::store_kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(B)),
-                         dim3(256), 0, static_cast<cudaStream_t>(stream), true, b, p),
+                         dim3(256), plan_smem(0, b), static_cast<cudaStream_t>(stream), true, b, p),
                   "tk_cache_store launch");
 }
 

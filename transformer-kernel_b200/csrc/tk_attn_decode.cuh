@@ -440,6 +440,19 @@ __device__ __forceinline__ void take_states(const Params& p, const uint8_t* base
   }
 }
 
+// Whether another row names the same sequence: two new tokens for one place.
+// Each of `n` threads looks at every n-th row.
+__device__ __forceinline__ bool named_twice(const Params& p, int b, int slot, int t, int n) {
+  bool twice = false;
+  if (p.k_new != nullptr && p.slots != nullptr)
+    for (int i = t; i < p.B; i += n) twice |= i != b && p.slots[i] == slot;
+  if (twice) {
+    atomicOr(p.status, paged::kBadSlot);
+    report_error(kDevCacheRefused, 0xB600u + kSiteSlot);
+  }
+  return twice;
+}
+
 // WPS warps per segment (b, kv head, tile of up to 16 query heads): with 4 a
 // CTA has one segment, warp w takes steps w, w + 4, ... and the four results
 // meet in shared memory; with 1 each warp has its own and nothing is merged.
@@ -466,7 +479,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
   item /= p.gtiles;
   const int kvh = item % p.Hkv, b = item / p.Hkv;
   int slot, len;
-  const bool live = b < p.B && *p.status == 0 && row_ok(p, b, &slot, &len, WPS == 1 ? lane == 0 : threadIdx.x == 0);
+  const bool live = b < p.B && *p.status == 0 &&
+                    row_ok(p, b, &slot, &len, WPS == 1 ? lane == 0 : threadIdx.x == 0) &&
+                    !named_twice(p, b, slot, WPS == 1 ? lane : static_cast<int>(threadIdx.x), WPS * 32);
   // status may be set by another CTA of this launch: one answer for the segment
   if (WPS == 1 ? !__all_sync(0xffffffffu, live) : !__syncthreads_and(live)) return;
   const int h0 = kvh * p.G + gt * kRows, rows = min(kRows, p.G - gt * kRows);
@@ -612,6 +627,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
   __shared__ __align__(8) uint64_t full[kWarps][NST];
   __shared__ int64_t sh_first[kMaxRows + 1];  // steps of one segment each of the rows before
   __shared__ int sh_len[kMaxRows], sh_slot[kMaxRows];
+  __shared__ uint32_t sh_seen[paged::kMaxEntries / 32];  // sequences that get a new token
   __shared__ int64_t sh_sum[kWarps];
   __shared__ float sh_m[kWarps][kRows], sh_l[kWarps][kRows];
   __shared__ int sh_at[kWarps];
@@ -628,6 +644,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
   const int status = *p.status;
   if (__syncthreads_or(status)) return;  // join_kernel then returns as well
   const int segs = p.Hkv * p.gtiles;
+  const bool check_twice = p.k_new != nullptr && p.slots != nullptr;
+  if (check_twice) {
+    for (int i = threadIdx.x; i < (p.max_seqs + 31) / 32; i += kThreads) sh_seen[i] = 0u;
+    __syncthreads();
+  }
+  bool twice = false;
 
   // lengths and the exclusive prefix sum of the rows' steps
   int64_t carry = 0;
@@ -637,6 +659,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     int64_t x = 0;
     if (b < p.B) {
       if (!row_ok(p, b, &slot, &len, blockIdx.x == 0)) len = -1;  // left as it is
+      else if (check_twice) twice |= atomicOr(&sh_seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1u;
       x = len > 0 ? Span<KS>(p, len).steps : 0;
       sh_len[b] = len;
       sh_slot[b] = slot;
@@ -657,6 +680,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     }
     if (b < p.B) sh_first[b] = before + x - own;
     __syncthreads();
+  }
+  if (check_twice && __syncthreads_or(twice)) {  // in every CTA: two new tokens for one place
+    if (twice && blockIdx.x == 0) {
+      atomicOr(p.status, paged::kBadSlot);
+      report_error(kDevCacheRefused, 0xB600u + kSiteSlot);
+    }
+    return;
   }
   const int64_t total = carry * segs;
   // rows without keys: zeros for an empty sequence, nothing for the others

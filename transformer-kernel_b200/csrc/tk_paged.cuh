@@ -466,19 +466,36 @@ struct StoreParams {
 };
 
 __global__ void __launch_bounds__(256) store_kernel(Books b, StoreParams p) {
+  extern __shared__ int sh[];
+  uint32_t* seen = reinterpret_cast<uint32_t*>(sh);  // [max_seqs / 32]
+  for (int i = threadIdx.x; i < (b.max_seqs + 31) / 32; i += blockDim.x) seen[i] = 0u;
   grid_dep_wait();
-  if (*b.status != 0) return;
+  const int status = *b.status;  // only a refusal of this very list can set it meanwhile
+  if (__syncthreads_or(status)) return;
+  const int ps = 1 << b.page_shift;
+  // every CTA checks every row, so that all agree whether the call applies
+  int bad = 0;
+  for (int i = threadIdx.x; i < static_cast<int>(gridDim.y); i += blockDim.x) {
+    const int s = p.slots[i];
+    if (s == -1) continue;
+    if (s < 0 || s >= b.max_seqs) {
+      bad |= kBadSlot;
+      continue;
+    }
+    if (atomicOr(&seen[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u) bad |= kBadSlot;
+    const int count = p.counts == nullptr ? p.S : p.counts[i];
+    const int64_t len = b.lens[s];
+    if (count < 0 || count > p.S || count > len || len > b.width * ps) bad |= kTooLong;
+  }
+  if (__syncthreads_or(bad)) {
+    if (bad && blockIdx.x == 0 && blockIdx.y == 0) refuse(b, bad, 0xB500u);
+    return;
+  }
   const int row = blockIdx.y;
   const int s = p.slots[row];
   if (s == -1) return;
-  const int ps = 1 << b.page_shift;
-  const bool slot_ok = s >= 0 && s < b.max_seqs;
   const int count = p.counts == nullptr ? p.S : p.counts[row];
-  const int64_t len = slot_ok ? b.lens[s] : 0;
-  if (!slot_ok || count < 0 || count > p.S || count > len || len > b.width * ps) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) refuse(b, slot_ok ? kTooLong : kBadSlot, 0xB500u);
-    return;
-  }
+  const int64_t len = b.lens[s];
   const int per_token = p.heads * p.row_vecs;
   const int64_t total = static_cast<int64_t>(count) * per_token;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
