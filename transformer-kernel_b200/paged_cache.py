@@ -155,8 +155,8 @@ class PagedCache:
         return self._books.clone()
 
     def restore(self, saved: torch.Tensor) -> None:
-        if saved.shape != self._books.shape or saved.dtype != torch.int32:
-            raise ValueError("not a snapshot of a cache of these sizes")
+        if saved.shape != self._books.shape or saved.dtype != torch.int32 or saved.device != self.device:
+            raise ValueError("not a snapshot of a cache of these sizes on this device")
         self._books.copy_(saved)
 
     def check(self) -> None:
@@ -215,17 +215,26 @@ class PagedCache:
         ``k`` and ``v`` are logically ``[B, kv_heads, S, head_dim]`` fp16 with
         the same strides and a contiguous last dimension, e.g. views of the
         fused QKV projection; token t >= counts[b] is padding."""
-        if k.dim() != 4 or k.shape != v.shape or k.shape[1] != self.kv_heads or k.shape[3] != self.head_dim:
+        shape = k.shape
+        if len(shape) != 4 or v.shape != shape or shape[1] != self.kv_heads or shape[3] != self.head_dim:
             raise ValueError(f"k/v must be [B, {self.kv_heads}, S, {self.head_dim}], got {tuple(k.shape)} and "
                              f"{tuple(v.shape)}")
-        self._check_data("store", k, v)
-        s = self._slots(slots)
-        c = None if counts is None else self._ints(counts, "counts")
-        if s.numel() != k.shape[0] or (c is not None and c.numel() != k.shape[0]):
-            raise ValueError(f"{k.shape[0]} rows, but {s.numel()} slots"
-                             + ("" if c is None else f" and {c.numel()} counts"))
-        self._call("tk_cache_store", int(layer), k.data_ptr(), v.data_ptr(), *k.stride()[:3],
-                   s.data_ptr(), tk.ptr(c), k.shape[0], k.shape[2])
+        B, _, S, _ = shape
+        k_b, k_h, k_s, k_1 = strides = k.stride()
+        if (not (k.dtype == v.dtype == torch.float16) or not (k.device == v.device == self.device) or k_1 != 1
+                or v.stride() != strides):
+            self._check_data("store", k, v)
+        slots = self._slots(slots)
+        if slots.numel() != B:
+            raise ValueError(f"{B} rows, but {slots.numel()} slots")
+        counts_ptr = None
+        if counts is not None:
+            counts = self._ints(counts, "counts")
+            if counts.numel() != B:
+                raise ValueError(f"{B} rows, but {counts.numel()} counts")
+            counts_ptr = counts.data_ptr()
+        self._call("tk_cache_store", layer, k.data_ptr(), v.data_ptr(), k_b, k_h, k_s, slots.data_ptr(), counts_ptr,
+                   B, S)
 
     def attend(
         self,
