@@ -592,6 +592,24 @@ def test_decode_every_division_of_the_work(cuda_device, head_dim, kv_heads, head
 
 
 @gpu
+@pytest.mark.parametrize("max_len", [0, 300])
+def test_decode_more_rows_than_the_split_takes(cuda_device, max_len):
+    """700 rows read three sequences (without new tokens that is allowed): too
+    many rows to be split, in a wide table a CTA and below a bound a warp each."""
+    cache, kv, g = filled([290, 1, 77], 16, 2, 64, width=400)
+    q = torch.randn(700, 4, 64, generator=g, device="cuda").half()
+    slots = (torch.arange(700, device="cuda") % 3).int()
+    out = cache.attend(0, q, 0.125, slots=slots, max_len=max_len).view(700, 4, 64)
+    for s in range(3):
+        rows = torch.arange(s, 700, 3, device="cuda")
+        for b in rows[::29].tolist():
+            ref, tol = attend_reference(q[b], kv[s][0], kv[s][1], 0.125)
+            assert bool(((out[b].double() - ref).abs() <= tol).all())
+    assert bool(torch.isfinite(out).all())
+    cache.check()
+
+
+@gpu
 def test_decode_one_long_sequence_over_the_whole_gpu(cuda_device):
     """One key-value head, 50,000 keys: hundreds of parts joined in order."""
     cache, kv, g = filled([50000], 64, 1, 64)
