@@ -786,3 +786,47 @@ def test_another_stream_and_two_devices_worth_of_handles(cuda_device):
                 c.attend(0, q, 0.125, out=o)
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+@gpu
+@pytest.mark.parametrize("pairs, ps", [(33, 16), (64, 32), (513, 16), (1000, 16), (4000, 16)])
+def test_many_forks_follow_the_model(cuda_device, pairs, ps):
+    """More pairs than a warp, and than the planning CTA, has threads. Parents
+    end inside or at the end of a page or are empty, some entries are padding,
+    and pages handed out are far fewer than pairs in half of the rounds: the
+    whole table, lengths, references and every copied row are the model's."""
+    g = torch.Generator().manual_seed(pairs)
+    for round_ in range(4):
+        parents_n = max(1, pairs // 3)
+        if round_ == 0:    # whole pages first, then partial ones
+            lens = [ps * 2] * (parents_n // 2) + [ps + 1 + i % (ps - 1) for i in range(parents_n - parents_n // 2)]
+        elif round_ == 1:  # one partial page in sixteen
+            lens = [ps * (1 + i % 3) - (i % 16 == 5) for i in range(parents_n)]
+        else:
+            lens = torch.randint(0, 3 * ps + 1, (parents_n,), generator=g).tolist()
+        used = sum(-(-n // ps) for n in lens)
+        cache, model = make(num_pages=used + pairs + 5, page_size=ps, max_seqs=parents_n + pairs, width=3, layers=2,
+                            kv_heads=1, head_dim=8)
+        dev_g = torch.Generator(device="cuda").manual_seed(round_)
+        cache.pages.copy_(torch.randn(cache.pages.shape, generator=dev_g, device="cuda").half())
+        slots = list(range(parents_n))
+        cache.reserve(slots, lens)
+        model.reserve(slots, lens)
+        parents = sorted(int(x) for x in torch.randint(0, parents_n, (pairs,), generator=g))
+        children = (torch.randperm(pairs, generator=g) + parents_n).tolist()
+        for i in range(0, pairs, 7):
+            if i % 2:
+                parents[i] = -1
+            else:
+                children[i] = -1
+        want = cache.pages.clone()
+        copies = model.fork(parents, children)
+        cache.fork(ints(*parents), ints(*children))
+        cache.check()
+        same_books(cache, model)
+        if copies:
+            src, dst, rows = (torch.tensor(x, device="cuda") for x in zip(*copies))
+            for n in range(1, ps):
+                at = rows == n
+                want[:, dst[at], :, :, :n] = want[:, src[at], :, :, :n]
+        torch.testing.assert_close(cache.pages, want, rtol=0, atol=0)

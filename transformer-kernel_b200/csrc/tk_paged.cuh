@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     b.table[dst[i] * b.width + (b.lens[src[i]] >> b.page_shift)] = page;
     take_page(b, page);
   }
+  __syncthreads();  // the owners have been looked up: `first` now takes the lengths
   // a child may be another pair's (empty) parent: every length is read before any is written
   for (int i0 = 0; i0 < n; i0 += blockDim.x) {
     const int i = i0 + static_cast<int>(threadIdx.x);
