@@ -182,3 +182,60 @@ def test_serving_refuses_on_device(cuda_device):
     cache.reset()
     assert model.decode_step(x[:0, 0], cache, []).shape == (0, 128)
     cache.check()
+
+
+def test_mask_lengths_follow_the_mask():
+    """A mask tensor that is filled again is read again; one that is not keeps
+    its lengths (no second look at the device)."""
+    model = make_model()
+    mask = torch.tensor([[1, 1, 0, 0], [1, 0, 0, 0]], dtype=torch.bool)
+    first = model._prefix_lengths(mask)
+    assert first.tolist() == [2, 1]
+    assert model._prefix_lengths(mask) is first
+    mask[0, 2] = True
+    assert model._prefix_lengths(mask).tolist() == [3, 1]
+    mask.fill_(True)
+    assert model._prefix_lengths(mask) is None
+    mask.copy_(torch.tensor([[1, 0, 0, 0], [0, 0, 0, 0]]))
+    assert model._prefix_lengths(mask).tolist() == [1, 0]
+    with torch.inference_mode():  # such tensors do not count their changes
+        mask = torch.tensor([[1, 1, 0, 0]], dtype=torch.bool)
+        assert model._prefix_lengths(mask).tolist() == [2]
+        mask[0, 2] = True
+        assert model._prefix_lengths(mask).tolist() == [3]
+
+
+@gpu
+def test_prefill_reads_a_mask_that_is_filled_again(cuda_device):
+    """One mask buffer for every batch, refilled by torch operations and by a
+    replayed graph: each prompt's own length reaches the cache and the output."""
+    model = make_model(d=128, heads=4).cuda()
+    g = torch.Generator().manual_seed(7)
+    S = 24
+    x = torch.randn(2, S, 128, generator=g).cuda()
+    mask, fresh = (torch.zeros(2, S, dtype=torch.bool, device="cuda") for _ in range(2))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mask.copy_(fresh)
+    cache = make_cache(model)
+    with torch.inference_mode():
+        want = [stack(model, s) for s in x]
+    for round_, lens in enumerate(([24, 5], [7, 24], [1, 2], [24, 24])):
+        now = (torch.arange(S)[None, :] < torch.tensor(lens)[:, None]).cuda()
+        if round_ % 2:
+            fresh.copy_(now)
+            graph.replay()
+        else:
+            mask.copy_(now)
+        slots = [2 * round_, 2 * round_ + 1]
+        with torch.no_grad():
+            out = model.prefill(x, cache, slots, mask)
+        assert cache.seq_lens[slots].tolist() == lens
+        for b, n in enumerate(lens):
+            agrees(out[b, :n], want[b][:n])
+    cache.check()
+    with pytest.raises(tk.TKError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            model.prefill(x, cache, [0, 1], mask)
+    assert cache.seq_lens.tolist() == [24, 5, 7, 24, 1, 2, 24, 24]
+    cache.check()

@@ -174,6 +174,7 @@ class OptimizedTransformer(nn.Module):
         self._mask_ref: Optional[weakref.ReferenceType] = None
         self._mask_lengths: Optional[torch.Tensor] = None  # None = dense
         self._mask_key: Optional[tuple] = None
+        self._mask_version: Optional[int] = None
         # Optional launch trace: a list that receives (name, start, end)
         # CUDA events around every kernel launch of the next forwards.
         self.launch_trace: Optional[list] = None
@@ -248,8 +249,12 @@ class OptimizedTransformer(nn.Module):
     @_outside_compile
     def _prefix_lengths(self, mask: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
         """``None`` for an all-True (or absent) mask, else the int32 per-row
-        prefix lengths. One device->host sync per distinct mask object
-        (weakref memo, like the reference's ``_mask_is_dense``, :362-389).
+        prefix lengths. One device->host sync per distinct mask object and
+        change to it (weakref memo, like the reference's ``_mask_is_dense``,
+        :362-389, checked against the tensor's version counter, which every
+        torch operation that writes the mask moves; writes that torch does not
+        see, such as a replayed graph's, need a new tensor). Tensors without a
+        counter, those made in inference mode, are read at every call.
         Masks that are not per-row prefixes -- the only kind the harness's
         ``generate_random_case`` makes (:261-271) -- raise."""
         return self._prefix_lengths_keyed(mask)[0]
@@ -259,21 +264,27 @@ class OptimizedTransformer(nn.Module):
         lengths' values (None when dense), taken at the same sync."""
         if mask is None or self.settings.assume_dense_mask:
             return None, None
-        if self._mask_ref is not None and self._mask_ref() is mask:
+        version = None if mask.is_inference() else mask._version
+        if (version is not None and self._mask_ref is not None and self._mask_ref() is mask
+                and self._mask_version == version):
             return self._mask_lengths, self._mask_key
+        result, key = self._count_prefixes(mask)
+        self._mask_ref, self._mask_version = weakref.ref(mask), version
+        self._mask_lengths, self._mask_key = result, key
+        return result, key
+
+    @staticmethod
+    def _count_prefixes(mask: torch.Tensor):
+        """(lengths, key) of what the mask holds now."""
         m = mask.to(torch.bool)
         lengths = m.sum(dim=-1, dtype=torch.int32)
         if bool(m.all()):
-            result, key = None, None
-        else:
-            prefix = torch.arange(m.shape[-1], device=m.device)[None, :] < lengths[:, None]
-            if not bool((prefix == m).all()):
-                raise tk.TKError("forward", -2, "valid_token_mask must be a per-row prefix (True then False)")
-            result = lengths.contiguous()
-            key = tuple(result.tolist())
-        self._mask_ref = weakref.ref(mask)
-        self._mask_lengths, self._mask_key = result, key
-        return result, key
+            return None, None
+        prefix = torch.arange(m.shape[-1], device=m.device)[None, :] < lengths[:, None]
+        if not bool((prefix == m).all()):
+            raise tk.TKError("forward", -2, "valid_token_mask must be a per-row prefix (True then False)")
+        result = lengths.contiguous()
+        return result, tuple(result.tolist())
 
     # -- forward --------------------------------------------------------------
     # The forward is opaque to torch.compile (the harness's --compile-user
@@ -468,13 +479,20 @@ class OptimizedTransformer(nn.Module):
         """``forward`` over prompts, which also fills the empty ``slots`` of
         the cache (row b's valid tokens go to ``slots[b]``). With ``window`` >
         0 a token sees the ``window`` latest keys and the first ``sinks``
-        ones. Returns ``[B, S, d]`` in x's dtype."""
+        ones. Returns ``[B, S, d]`` in x's dtype. The mask is read as it is at
+        this call, which waits for the device; with one, ``prefill`` cannot be
+        captured into a CUDA graph."""
         self._check_input(x)
         self._check_cache(cache, x.device, window, sinks)
         B, S, d = x.shape
         if B * S == 0:
             raise ValueError(f"prompts need at least one row and one token, got {tuple(x.shape)}")
-        lengths = self._prefix_lengths(valid_token_mask)
+        lengths = None
+        if valid_token_mask is not None and not self.settings.assume_dense_mask:
+            if torch.cuda.is_current_stream_capturing():
+                raise tk.TKError("prefill", -2, "the lengths of a mask cannot be read while a CUDA graph is captured")
+            # the lengths go into the cache's books: never those of an earlier call
+            lengths, _ = self._count_prefixes(valid_token_mask)
         counts = torch.full((B,), S, dtype=torch.int32, device=x.device) if lengths is None else lengths
         slots = cache._slots(slots)
         cache.reserve(slots, counts, require_empty=True)
