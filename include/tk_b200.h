@@ -266,8 +266,8 @@ TK_API int tk_copy_rows(void* dst, int64_t dst_ld, const void* src, int64_t src_
  * nothing changes, the status word and the device error word are set, and
  * until the caller zeroes the status word later calls on the cache do nothing
  * (tk_attn_decode then leaves its output as it is). tk_attn_decode reports a
- * slot or a length that cannot be the same way; that call's output is then
- * unspecified. Slot lists are int32 on the device, at most 8192 entries, each
+ * slot or a length that cannot be the same way: none of the call's new tokens
+ * is stored, its output is unspecified. Slot lists are int32 on the device, at most 8192 entries, each
  * slot at most once; slot -1 is padding. Calls on one cache must be ordered on
  * the GPU. */
 typedef struct tk_cache {

@@ -830,3 +830,42 @@ def test_many_forks_follow_the_model(cuda_device, pairs, ps):
                 at = rows == n
                 want[:, dst[at], :, :, :n] = want[:, src[at], :, :, :n]
         torch.testing.assert_close(cache.pages, want, rtol=0, atol=0)
+
+
+@gpu
+@pytest.mark.parametrize("rows, kv_heads, width", [(64, 2, 3), (80, 16, 3), (9, 2, 400)])
+@pytest.mark.parametrize("fault, bit", [("twice", 2), ("slot", 2), ("too long", 4), ("negative", 4)])
+@pytest.mark.parametrize("at", [0, -1])
+def test_decode_with_new_tokens_applies_whole_or_not_at_all(cuda_device, rows, kv_heads, width, fault, bit, at):
+    """One row that cannot be, first or last in the list, in every division of
+    the work: no row's token is stored; the same call without the fault
+    applies to all rows."""
+    cache, kv, g = filled([40] * rows, 16, kv_heads, 64, width=width)
+    before = cache.pages.clone()
+    q = torch.randn(rows, kv_heads, 64, generator=g, device="cuda").half()
+    new = torch.randn(2, rows, kv_heads, 64, generator=g, device="cuda").half()
+    slots = torch.arange(rows, dtype=torch.int32, device="cuda")
+    out = torch.full((rows, kv_heads * 64), 7.0, device="cuda").half()
+    saved = cache.snapshot()
+    if fault == "twice":
+        slots[at] = rows // 2
+    elif fault == "slot":
+        slots[at] = rows
+    else:
+        cache.seq_lens[at] = 10 ** 6 if fault == "too long" else -3
+    cache.attend(0, q, 0.125, k_new=new[0], v_new=new[1], slots=slots, out=out)
+    assert int(cache.status) == bit
+    assert torch.equal(cache.pages.view(torch.int16), before.view(torch.int16))
+    with pytest.raises(tk.TKError):
+        tk.check_device_errors(cuda_device)
+    cache.restore(saved)
+    slots.copy_(torch.arange(rows))
+    cache.attend(0, q, 0.125, k_new=new[0], v_new=new[1], slots=slots, out=out)
+    cache.check()
+    page = cache.page_table[:, 2].long()
+    assert torch.equal(cache.pages[0, page, 0, :, 7], new[0]) and torch.equal(cache.pages[0, page, 1, :, 7], new[1])
+    for b in (0, rows // 2, rows - 1):
+        k = torch.cat([kv[b][0][:, :-1], new[0][b][:, None]], 1)
+        v = torch.cat([kv[b][1][:, :-1], new[1][b][:, None]], 1)
+        ref, tol = attend_reference(q[b], k, v, 0.125)
+        assert bool(((out[b].view(kv_heads, 64).double() - ref).abs() <= tol).all())

@@ -1081,12 +1081,22 @@ int launch_decode(DeviceInfo* info, int slot, tk::decode::Params& p, int64_t pag
     }
   }
   const int64_t segments = static_cast<int64_t>(p.B) * p.Hkv * p.gtiles;
+  if (how != kSplit && p.k_new != nullptr) {
+    // a 16-byte piece of keys and of values a thread, fewer CTAs where they
+    // would not fit into the first wave
+    const int64_t vecs = static_cast<int64_t>(p.B) * p.Hkv * (p.hd / 8);
+    const int64_t room = static_cast<int64_t>(info->sms) * C::CTAS - (how == kWarpEach ? (segments + 3) / 4 : segments);
+    int64_t ctas = std::min<int64_t>((vecs + 127) / 128, info->sms);
+    if (room > 0 && ctas > room) ctas = std::max<int64_t>(room, std::min<int64_t>((vecs + 1023) / 1024, info->sms));
+    p.store_ctas = static_cast<int>(ctas);
+  }
   if (how == kWarpEach)
-    return launched(launch(tk::decode::decode_kernel<HD, TWO, 1>, dim3(static_cast<unsigned>((segments + 3) / 4)),
+    return launched(launch(tk::decode::decode_kernel<HD, TWO, 1>,
+                           dim3(static_cast<unsigned>(p.store_ctas + (segments + 3) / 4)),
                            dim3(tk::decode::kThreads), C::SMEM_BYTES, s, true, mk, mv, p),
                     "tk_attn_decode launch");
   if (how == kCtaEach)
-    return launched(launch(tk::decode::decode_kernel<HD, TWO, 4>, dim3(static_cast<unsigned>(segments)),
+    return launched(launch(tk::decode::decode_kernel<HD, TWO, 4>, dim3(static_cast<unsigned>(p.store_ctas + segments)),
                            dim3(tk::decode::kThreads), C::SMEM_BYTES, s, true, mk, mv, p),
                     "tk_attn_decode launch");
   if (workspace_bytes < split_bytes<HD>(info->sms))
@@ -1291,7 +1301,7 @@ int tk_attn_decode(const tk_cache* cache, int64_t layer, const void* q, int64_t 
   if (ld_out < H * cache->hd || ld_out % 2 || !aligned(out, 4))
     return fail(TK_ERR_INVALID, "tk_attn_decode: out needs 4-byte aligned rows and ld_out >= H*hd");
   const int64_t G = H / cache->kv_heads, gtiles = (G + tk::decode::kRows - 1) / tk::decode::kRows;
-  if (B * cache->kv_heads * gtiles > (1ll << 31) - 1)
+  if (B * cache->kv_heads * gtiles > (1ll << 31) - 1024)
     return fail(TK_ERR_UNSUPPORTED, "tk_attn_decode: grid too large");
   int dev;
   DeviceInfo* info;
@@ -1349,6 +1359,7 @@ int tk_attn_decode(const tk_cache* cache, int64_t layer, const void* q, int64_t 
   if (can_split && (span > 4096 || (span >= 2048 && segments < info->sms))) how = kSplit;
   else if (segments >= 3 * info->sms && span <= 2048) how = kWarpEach;
   p.min_steps = 8;
+  p.store_ctas = 0;
   if (how == kSplit && !aligned(workspace, 256))
     return fail(TK_ERR_INVALID, "tk_attn_decode: the workspace needs 256-byte alignment");
   auto run = [&](auto launch_two, auto launch_one, int slot) {

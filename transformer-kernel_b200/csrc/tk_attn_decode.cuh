@@ -91,6 +91,7 @@ struct Params {
   int window, sinks;      // window 0: every key
   float scale_log2;
   uint64_t wait_limit_ns;
+  int store_ctas;         // first CTAs of decode_kernel: they store the new tokens (none without k_new)
   // split over the grid (decode_split_kernel)
   int ctas, min_steps;    // CTAs of the grid; fewest steps one takes
   int2* info;             // [B * Hkv * gtiles]: first CTA and number of parts of a split result, (0, 0) if whole
@@ -442,28 +443,70 @@ __device__ __forceinline__ void take_states(const Params& p, const uint8_t* base
   }
 }
 
-// Whether another row names the same sequence: two new tokens for one place.
-// Each of `n` threads looks at every n-th row.
-__device__ __forceinline__ bool named_twice(const Params& p, int b, int slot, int t, int n) {
-  bool twice = false;
-  if (p.k_new != nullptr && p.slots != nullptr)
-    for (int i = t; i < p.B; i += n) twice |= i != b && p.slots[i] == slot;
-  if (twice) {
-    atomicOr(p.status, paged::kBadSlot);
-    report_error(kDevCacheRefused, 0xB600u + kSiteSlot);
+// The new tokens of a call are stored whole or not at all, by CTAs of their own:
+// each looks at every row first -- a slot or a length that cannot be, a sequence
+// that two rows name (two new tokens for one place) -- so that all agree, and no
+// segment waits for that. The segments take the new token from the argument and
+// never see what its place in the page holds. `seen`: a bit per sequence.
+// (Checks in every segment's CTA instead: 256 short sequences, 16 heads of 64,
+// 29.4 us against 28.6; 1000 of 30 tokens, 4 heads of 32, 15.0 against 7.3.)
+__device__ __forceinline__ void store_new_rows(const Params& p, uint32_t* seen) {
+  for (int i = threadIdx.x; i < (p.max_seqs + 31) / 32; i += kThreads) seen[i] = 0u;
+  grid_dep_wait();
+  const int status = *p.status;
+  if (__syncthreads_or(status)) return;
+  int bad = 0;
+  for (int i = threadIdx.x; i < p.B; i += kThreads) {
+    const int s = p.slots == nullptr ? i : p.slots[i];
+    if (s == -1) continue;
+    if (s < 0 || s >= p.max_seqs) {
+      bad |= paged::kBadSlot;
+      continue;
+    }
+    if (atomicOr(&seen[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u) bad |= paged::kBadSlot;
+    const int len = p.lens[s];
+    if (len < 0 || len > (p.width << p.page_shift)) bad |= paged::kTooLong;
   }
-  return twice;
+  if (__syncthreads_or(bad)) {
+    if (bad) {
+      atomicOr(p.status, bad);
+      report_error(kDevCacheRefused, 0xB600u + ((bad & paged::kBadSlot) ? kSiteSlot : kSiteLen));
+    }
+    return;
+  }
+  const int vecs = p.hd / 8, per_row = p.Hkv * vecs, in_page = (1 << p.page_shift) - 1;
+  const int64_t total = static_cast<int64_t>(p.B) * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
+       i += static_cast<int64_t>(p.store_ctas) * kThreads) {
+    const int b = static_cast<int>(i / per_row), within = static_cast<int>(i % per_row);
+    const int h = within / vecs, c = within % vecs;
+    const int s = p.slots == nullptr ? b : p.slots[b];
+    if (s == -1) continue;
+    const int last = p.lens[s] - 1;
+    if (last < 0) continue;
+    const int page = p.table[s * p.width + (last >> p.page_shift)];
+    if (page < 0 || page >= p.num_pages) continue;  // reported by the segment that reads it
+    const int64_t from = b * p.new_stride_b + h * p.new_stride_h + c * 8;
+    const int64_t to = page * p.page_stride + h * p.head_stride + static_cast<int64_t>(last & in_page) * p.hd + c * 8;
+    *reinterpret_cast<uint4*>(p.k_pages + to) = *reinterpret_cast<const uint4*>(p.k_new + from);
+    *reinterpret_cast<uint4*>(p.v_pages + to) = *reinterpret_cast<const uint4*>(p.v_new + from);
+  }
 }
 
 // WPS warps per segment (b, kv head, tile of up to 16 query heads): with 4 a
 // CTA has one segment, warp w takes steps w, w + 4, ... and the four results
 // meet in shared memory; with 1 each warp has its own and nothing is merged.
+// With new tokens the grid's first store_ctas CTAs store them.
 template <int HD, bool TWO, int WPS>
 __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Params p) {
   using C = Cfg<HD>;
   constexpr int KS = C::KS, NST = C::NST;
   extern __shared__ uint8_t smem_raw[];
+  if (blockIdx.x < static_cast<unsigned>(p.store_ctas)) {
+    store_new_rows(p, reinterpret_cast<uint32_t*>(smem_raw));
+    return;
+  }
   __shared__ __align__(8) uint64_t full[kWarps][NST];
   __shared__ float sh_m[kWarps][kRows], sh_l[kWarps][kRows];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -476,14 +519,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
   }
   __syncwarp();
   grid_dep_wait();
-  int item = WPS == 1 ? blockIdx.x * kWarps + warp : blockIdx.x;
+  const int cta = static_cast<int>(blockIdx.x) - p.store_ctas;
+  int item = WPS == 1 ? cta * kWarps + warp : cta;
   const int gt = item % p.gtiles;
   item /= p.gtiles;
   const int kvh = item % p.Hkv, b = item / p.Hkv;
-  int slot, len;
-  const bool live = b < p.B && *p.status == 0 &&
-                    row_ok(p, b, &slot, &len, WPS == 1 ? lane == 0 : threadIdx.x == 0) &&
-                    !named_twice(p, b, slot, WPS == 1 ? lane : static_cast<int>(threadIdx.x), WPS * 32);
+  int slot = -1, len = 0;
+  bool live = false;
+  if (b < p.B && *p.status == 0) live = row_ok(p, b, &slot, &len, WPS == 1 ? lane == 0 : threadIdx.x == 0);
   // status may be set by another CTA of this launch: one answer for the segment
   if (WPS == 1 ? !__all_sync(0xffffffffu, live) : !__syncthreads_and(live)) return;
   const int h0 = kvh * p.G + gt * kRows, rows = min(kRows, p.G - gt * kRows);
@@ -532,16 +575,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     // let copies already in flight land before the CTA can exit
     for (int i = max(0, loaded - NST); i < loaded; ++i)
       mbar_wait_warp(&full[warp][i % NST], (i / NST) & 1, nullptr, kDrainLimitNs);
-  } else if (has_new && gt == 0) {
-    // pg still holds the page of the last step (16 keys per number)
-    const int part = (len - 1 - sp.key0(sp.steps - 1)) / 16;
-    int page = -1;
-#pragma unroll
-    for (int i = 0; i < KS / 16; ++i) {
-      const int id = __shfl_sync(0xffffffffu, pg.ids[i], (mine - 1) % 32);
-      if (i == part) page = id;
-    }
-    new_row.store(p, page, len, kvh);
   }
   grid_dep_launch();
   if (__any_sync(0xffffffffu, bad) && lane == 0) {
@@ -651,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     for (int i = threadIdx.x; i < (p.max_seqs + 31) / 32; i += kThreads) sh_seen[i] = 0u;
     __syncthreads();
   }
-  bool twice = false;
+  bool twice = false, wrong = false;
 
   // lengths and the exclusive prefix sum of the rows' steps
   int64_t carry = 0;
@@ -660,8 +693,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     int slot = -1, len = 0;
     int64_t x = 0;
     if (b < p.B) {
-      if (!row_ok(p, b, &slot, &len, blockIdx.x == 0)) len = -1;  // left as it is
-      else if (check_twice) twice |= atomicOr(&sh_seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1u;
+      if (!row_ok(p, b, &slot, &len, blockIdx.x == 0)) {
+        len = -1;  // left as it is
+        wrong |= slot != -1;
+      } else if (check_twice) twice |= atomicOr(&sh_seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1u;
       x = len > 0 ? Span<KS>(p, len).steps : 0;
       sh_len[b] = len;
       sh_slot[b] = slot;
@@ -683,7 +718,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     if (b < p.B) sh_first[b] = before + x - own;
     __syncthreads();
   }
-  if (check_twice && __syncthreads_or(twice)) {  // in every CTA: two new tokens for one place
+  // in every CTA: a row that cannot be, two new tokens for one place
+  if (p.k_new != nullptr && __syncthreads_or(twice || wrong)) {
     if (twice && blockIdx.x == 0) {
       atomicOr(p.status, paged::kBadSlot);
       report_error(kDevCacheRefused, 0xB600u + kSiteSlot);
