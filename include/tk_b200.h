@@ -288,7 +288,8 @@ typedef enum tk_cache_status {
   TK_CACHE_TOO_LONG = 4,      /* longer than the slot's row of the page table     */
   TK_CACHE_BAD_PAGE = 8,      /* the page table names a page outside the pool     */
   TK_CACHE_NOT_EMPTY = 16,    /* a slot that has to be empty is not               */
-  TK_CACHE_TIMED_OUT = 32     /* a wait inside an attention call gave up          */
+  TK_CACHE_TIMED_OUT = 32     /* a wait inside an attention call gave up: its output
+                                 and its new tokens are unspecified              */
 } tk_cache_status;
 
 /* Sequence slots[i] grows by counts[i] tokens and takes the pages that they
@@ -356,7 +357,9 @@ TK_API int tk_attn_supported(int64_t head_dim);
 TK_API int tk_check_device_errors(void* stream);
 
 /* Limit, in nanoseconds, of every device-side wait in later launches
- * (default 2e9). Returns the previous value. */
+ * (default 2e9). Returns the previous value. With 0 every wait of
+ * tk_attn_decode for its keys gives up at once, so that what it then reports
+ * can be tested. */
 TK_API uint64_t tk_set_wait_limit_ns(uint64_t ns);
 
 /* Launch later launch-bound (small) kernels with programmatic stream

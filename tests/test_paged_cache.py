@@ -869,3 +869,34 @@ def test_decode_with_new_tokens_applies_whole_or_not_at_all(cuda_device, rows, k
         v = torch.cat([kv[b][1][:, :-1], new[1][b][:, None]], 1)
         ref, tol = attend_reference(q[b], k, v, 0.125)
         assert bool(((out[b].view(kv_heads, 64).double() - ref).abs() <= tol).all())
+
+
+@gpu
+@pytest.mark.parametrize("rows, kv_heads, width", [(64, 2, 3), (80, 16, 3), (9, 2, 400)])
+def test_decode_reports_a_wait_that_gave_up(cuda_device, rows, kv_heads, width):
+    """With no time to wait, in every division of the work: the status word
+    says so, no output is made from the keys that came, later calls do nothing,
+    and the context goes on."""
+    cache, kv, g = filled([40] * rows, 16, kv_heads, 64, width=width)
+    q = torch.randn(rows, kv_heads, 64, generator=g, device="cuda").half()
+    out = torch.full((rows, kv_heads * 64), 7.0, device="cuda").half()
+    saved = cache.snapshot()
+    old = tk.set_wait_limit_ns(0)
+    try:
+        cache.attend(0, q, 0.125, out=out)
+        assert int(cache.status) == 32
+    finally:
+        tk.set_wait_limit_ns(old)
+    assert bool((out == 7).all())
+    cache.attend(0, q, 0.125, out=out)
+    assert bool((out == 7).all())
+    with pytest.raises(tk.TKError, match="gave up"):
+        cache.check()
+    with pytest.raises(tk.TKError, match="timed out"):
+        tk.check_device_errors(cuda_device)
+    cache.restore(saved)
+    cache.attend(0, q, 0.125, out=out)
+    cache.check()
+    for b in (0, rows - 1):
+        ref, tol = attend_reference(q[b], kv[b][0], kv[b][1], 0.125)
+        assert bool(((out[b].view(kv_heads, 64).double() - ref).abs() <= tol).all())

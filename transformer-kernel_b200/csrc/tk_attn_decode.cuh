@@ -443,6 +443,13 @@ __device__ __forceinline__ void take_states(const Params& p, const uint8_t* base
   }
 }
 
+// A wait gave up: the call's output and new tokens are not what they should be,
+// so later calls stop at the status word until the caller has put things right.
+__device__ __forceinline__ void report_timeout(const Params& p) {
+  atomicOr(p.status, paged::kTimedOut);
+  report_error(kDevWaitTimeout, 0xB600u + kSiteFull);
+}
+
 // The new tokens of a call are stored whole or not at all, by CTAs of their own:
 // each looks at every row first -- a slot or a length that cannot be, a sequence
 // that two rows name (two new tokens for one place) -- so that all agree, and no
@@ -537,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
 
   uint8_t* ring = smem + warp * NST * C::STAGE_BYTES;
   Pages<C> pg;
-  bool bad = false, ok = true;
+  bool bad = false, ok = mine == 0 || p.wait_limit_ns != 0;
   int loaded = 0;  // steps requested so far
   auto request = [&]() {
     if (loaded % 32 == 0) {
@@ -556,13 +563,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
   if (has_new) new_row.load(p, b, kvh);
   State<HD> st;
   st.reset();
-  for (int i = 0; i < mine; ++i) {
+  for (int i = 0; ok && i < mine; ++i) {
     const int s = i % NST;
-    if (!mbar_wait_warp(&full[warp][s], (i / NST) & 1, nullptr, p.wait_limit_ns)) {
-      if (lane == 0) report_error(kDevWaitTimeout, 0xB600u + kSiteFull);
-      ok = false;
-      break;
-    }
+    ok = mbar_wait_warp(&full[warp][s], (i / NST) & 1, nullptr, p.wait_limit_ns);
+    if (!ok) break;
     uint8_t* stage = ring + s * C::STAGE_BYTES;
     const int key0 = sp.key0(first + i * WPS);
     const bool whole = sp.whole(key0);
@@ -572,6 +576,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     if (loaded < mine) request();
   }
   if (!ok) {
+    if (lane == 0) report_timeout(p);
     // let copies already in flight land before the CTA can exit
     for (int i = max(0, loaded - NST); i < loaded; ++i)
       mbar_wait_warp(&full[warp][i % NST], (i / NST) & 1, nullptr, kDrainLimitNs);
@@ -582,6 +587,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     report_error(kDevCacheRefused, 0xB600u + kSitePage);
   }
   if (WPS == 1) {
+    if (!ok) return;
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int r = 0; r < (TWO ? 2 : 1); ++r) {
@@ -600,7 +606,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     }
     return;
   }
-  __syncthreads();  // every warp is done with its ring, which the merge reuses
+  // every warp is done with its ring, which the merge reuses, and has seen all its keys
+  if (!__syncthreads_and(ok)) return;
   put_state<C, TWO>(st, reinterpret_cast<float*>(ring), sh_m[warp], sh_l[warp]);
   __syncthreads();
   take_states<C>(p, smem, NST * C::STAGE_BYTES, nullptr, sh_m, sh_l, rows, [&](int rr, int c, float, float l, float2 o) {
@@ -767,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
   uint8_t* ring = smem + warp * NST * C::STAGE_BYTES;
   Pages<C> pg;
   int pg_b = -1, pg_step = 0;  // row and first step whose pages pg holds (every fourth step)
-  bool bad = false, ok = true;
+  bool bad = false, ok = p.wait_limit_ns != 0;
   int loaded = 0, used = 0;
   auto request = [&]() {
     const int ahead = get_step - pg_step;
@@ -806,13 +813,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     bool hold = false;
     for (int step = use.s0 + warp; step < use.s1; step += kWarps) {
       const int s = used % NST;
-      if (ok && !mbar_wait_warp(&full[warp][s], (used / NST) & 1, nullptr, p.wait_limit_ns)) {
-        if (lane == 0) {
-          atomicOr(p.status, paged::kTimedOut);  // join_kernel returns: parts are missing
-          report_error(kDevWaitTimeout, 0xB600u + kSiteFull);
-        }
-        ok = false;  // this warp only keeps the others company at the barriers now
-      }
+      // a warp that gave up only keeps the others company at the barriers
+      if (ok) ok = mbar_wait_warp(&full[warp][s], (used / NST) & 1, nullptr, p.wait_limit_ns);
       if (!ok) continue;
       ++used;
       uint8_t* stage = ring + s * C::STAGE_BYTES;
@@ -837,23 +839,24 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
       sh_m[warp][lane] = -INFINITY;
     }
     if (lane == 0) sh_at[warp] = held;
-    __syncthreads();
+    const bool all_ok = __syncthreads_and(ok);
     const bool begins = use.s0 == 0, ends = use.last();
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (begins ? 1 : 0);
-    take_states<C>(p, smem, NST * C::STAGE_BYTES, sh_at, sh_m, sh_l, rows,
-                   [&](int rr, int c, float m, float l, float2 o) {
-                     if (begins && ends) {
-                       const float inv = l > 0.f ? 1.f / l : 0.f;
-                       *reinterpret_cast<uint32_t*>(p.out + use.b * p.ld_out + (h0 + rr) * p.hd + c) =
-                           pack_half2(o.x * inv, o.y * inv);
-                     } else {
-                       if (c == 0) {
-                         p.part_ml[slot * 2 * kRows + rr] = m;
-                         p.part_ml[slot * 2 * kRows + kRows + rr] = l;
+    if (all_ok)
+      take_states<C>(p, smem, NST * C::STAGE_BYTES, sh_at, sh_m, sh_l, rows,
+                     [&](int rr, int c, float m, float l, float2 o) {
+                       if (begins && ends) {
+                         const float inv = l > 0.f ? 1.f / l : 0.f;
+                         *reinterpret_cast<uint32_t*>(p.out + use.b * p.ld_out + (h0 + rr) * p.hd + c) =
+                             pack_half2(o.x * inv, o.y * inv);
+                       } else {
+                         if (c == 0) {
+                           p.part_ml[slot * 2 * kRows + rr] = m;
+                           p.part_ml[slot * 2 * kRows + kRows + rr] = l;
+                         }
+                         *reinterpret_cast<float2*>(p.part_o + (slot * kRows + rr) * HD + c) = o;
                        }
-                       *reinterpret_cast<float2*>(p.part_o + (slot * kRows + rr) * HD + c) = o;
-                     }
-                   });
+                     });
     if (begins && threadIdx.x == 0) {
       const int parts = static_cast<int>((done + use.sp.steps - r0 + per - 1) / per);
       p.info[use.b * segs + use.sg] = ends ? make_int2(0, 0) : make_int2(blockIdx.x, parts);
@@ -863,6 +866,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::CTAS)
     if (hold && ok && more) request();
   }
   if (!ok) {
+    if (lane == 0) report_timeout(p);  // join_kernel returns: parts are missing
     // let copies already in flight land before the CTA can exit
     for (int i = max(0, loaded - NST); i < loaded; ++i)
       mbar_wait_warp(&full[warp][i % NST], (i / NST) & 1, nullptr, kDrainLimitNs);
