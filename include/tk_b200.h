@@ -286,7 +286,7 @@ typedef enum tk_cache_status {
   TK_CACHE_OUT_OF_PAGES = 1,  /* fewer free pages than the call needs             */
   TK_CACHE_BAD_SLOT = 2,      /* slot out of range or twice, or a negative count  */
   TK_CACHE_TOO_LONG = 4,      /* longer than the slot's row of the page table     */
-  TK_CACHE_BAD_PAGE = 8,      /* the page table names a page outside the pool     */
+  TK_CACHE_BAD_PAGE = 8,      /* the page table or a list names a page outside the pool */
   TK_CACHE_NOT_EMPTY = 16,    /* a slot that has to be empty is not               */
   TK_CACHE_TIMED_OUT = 32     /* a wait inside an attention call gave up: its output
                                  and its new tokens are unspecified              */

@@ -900,3 +900,28 @@ def test_decode_reports_a_wait_that_gave_up(cuda_device, rows, kv_heads, width):
     for b in (0, rows - 1):
         ref, tol = attend_reference(q[b], kv[b][0], kv[b][1], 0.125)
         assert bool(((out[b].view(kv_heads, 64).double() - ref).abs() <= tol).all())
+
+
+@gpu
+def test_copy_pages_applies_whole_or_not_at_all(cuda_device):
+    """A page outside the pool in the list: no page is copied; and a cache that
+    has refused a call copies nothing."""
+    cache, _ = make(num_pages=300, layers=2)
+    cache.pages.copy_(torch.arange(300, device="cuda").view(1, -1, 1, 1, 1, 1).expand(cache.pages.shape).half())
+    before, saved = cache.pages.clone(), cache.snapshot()
+    src, dst = list(range(100)), list(range(150, 250))
+    for at, pages, bad in ((99, "dst", 300), (0, "src", -1), (50, "dst", -5), (99, "src", 2 ** 30)):
+        s, d = ints(*src), ints(*dst)
+        (s if pages == "src" else d)[at] = bad
+        cache._call("tk_cache_copy_pages", s.data_ptr(), d.data_ptr(), 100)
+        assert int(cache.status) == 8 and torch.equal(cache.pages, before)
+        with pytest.raises(tk.TKError):
+            tk.check_device_errors(cuda_device)
+        cache.copy_pages(src, dst)  # refused before
+        assert int(cache.status) == 8 and torch.equal(cache.pages, before)
+        cache.restore(saved)
+    cache.copy_pages(src, dst)
+    before[:, dst] = before[:, src]
+    assert torch.equal(cache.pages, before)
+    cache.check()
+    tk.check_device_errors(cuda_device)

@@ -1208,7 +1208,7 @@ int tk_cache_copy_pages(const tk_cache* cache, const int32_t* src, const int32_t
   const int64_t vecs = pool.layers * pool.page_vecs;
   const int64_t chunks = std::min<int64_t>((vecs + 1023) / 1024, std::max<int64_t>(1, 8 * info->sms / n));
   return launched(launch(tk::paged::copy_pages_kernel, dim3(static_cast<unsigned>(n), static_cast<unsigned>(chunks)),
-                         dim3(256), 0, static_cast<cudaStream_t>(stream), true, pool, src, dst, b.num_pages),
+                         dim3(256), 0, static_cast<cudaStream_t>(stream), true, b, pool, src, dst),
                   "tk_cache_copy_pages launch");
 }
 

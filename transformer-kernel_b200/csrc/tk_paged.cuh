@@ -33,7 +33,7 @@ enum : int {
   kOutOfPages = 1,  // fewer free pages than the call needs
   kBadSlot = 2,     // a slot out of range or named twice, or a negative count
   kTooLong = 4,     // a sequence longer than its row of the page table
-  kBadPage = 8,     // the page table names a page outside the pool
+  kBadPage = 8,     // the page table or a list of pages names one outside the pool
   kNotEmpty = 16,   // a slot that has to be empty is not
   kTimedOut = 32,   // a wait inside an attention call gave up
 };
@@ -435,14 +435,20 @@ __global__ void __launch_bounds__(256) free_mask_kernel(Books b) {
   b.free_mask[w] = bits;
 }
 
-// Whole pages src[i] -> dst[i] of every layer; grid (pairs, chunks).
-__global__ void __launch_bounds__(256) copy_pages_kernel(Pool pool, const int* src, const int* dst, int num_pages) {
+// Whole pages src[i] -> dst[i] of every layer; grid (pairs, chunks). Every CTA
+// checks the whole list, so that all agree whether it applies.
+__global__ void __launch_bounds__(256) copy_pages_kernel(Books b, Pool pool, const int* src, const int* dst) {
   grid_dep_wait();
-  const int s = src[blockIdx.x], d = dst[blockIdx.x];
-  if (s < 0 || s >= num_pages || d < 0 || d >= num_pages) {
-    if (blockIdx.y == 0 && threadIdx.x == 0) report_error(kDevCacheRefused, 0xB400u);
+  const int status = *b.status;  // only a refusal of this very list can set it meanwhile
+  if (__syncthreads_or(status)) return;
+  int bad = 0;
+  for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += blockDim.x)
+    if (!page_ok(b, src[i]) || !page_ok(b, dst[i])) bad = kBadPage;
+  if (__syncthreads_or(bad)) {
+    if (bad && blockIdx.x == 0 && blockIdx.y == 0) refuse(b, bad, 0xB400u);
     return;
   }
+  const int s = src[blockIdx.x], d = dst[blockIdx.x];
   const int64_t total = pool.layers * pool.page_vecs;
   for (int64_t v = static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x; v < total;
        v += static_cast<int64_t>(gridDim.y) * blockDim.x) {

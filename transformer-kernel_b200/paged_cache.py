@@ -44,7 +44,7 @@ STATUS = {
     1: "out of pages",
     2: "a slot is out of range or named twice, or a count is negative",
     4: "a sequence is longer than its row of the page table, or has fewer tokens than the call stores",
-    8: "the page table names a page outside the pool",
+    8: "the page table or a list of pages names a page outside the pool",
     16: "a slot that has to be empty holds a sequence",
     32: "a device wait gave up",
 }
