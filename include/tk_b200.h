@@ -267,9 +267,15 @@ TK_API int tk_copy_rows(void* dst, int64_t dst_ld, const void* src, int64_t src_
  * until the caller zeroes the status word later calls on the cache do nothing
  * (tk_attn_decode then leaves its output as it is). tk_attn_decode reports a
  * slot or a length that cannot be the same way: none of the call's new tokens
- * is stored, its output is unspecified. Slot lists are int32 on the device, at most 8192 entries, each
- * slot at most once; slot -1 is padding. Calls on one cache must be ordered on
- * the GPU. */
+ * is stored, its output is unspecified. Only a page table that names pages
+ * outside the pool (books that these calls did not make) and a wait that gives
+ * up are found while a call already writes: tk_cache_fork, tk_cache_store and
+ * tk_attn_decode are reported then as well, but may have applied in part,
+ * always inside the pool. Slot lists are int32 on the device, at most 8192
+ * entries, each slot at most once (a fork's parents any number of times); slot
+ * -1 is padding. A fork shares full pages, so reserved tokens have to be stored
+ * before it: what is stored in a shared page is every holder's. Calls on one
+ * cache must be ordered on the GPU. */
 typedef struct tk_cache {
   int32_t* page_table;
   int32_t* seq_lens;

@@ -925,3 +925,27 @@ def test_copy_pages_applies_whole_or_not_at_all(cuda_device):
     assert torch.equal(cache.pages, before)
     cache.check()
     tk.check_device_errors(cuda_device)
+
+
+@gpu
+@pytest.mark.parametrize("page", [64, 10 ** 6, -7])
+def test_fork_and_store_report_pages_outside_the_pool(cuda_device, page):
+    """Books from elsewhere with such a page: the calls are reported, and write
+    nothing but what is theirs."""
+    cache, _ = make(layers=1, kv_heads=1, head_dim=16)
+    cache.reserve([0, 1, 2], [40, 40, 40])
+    cache.pages.fill_(1.0)
+    saved = cache.snapshot()
+    k = torch.full((2, 1, 40, 16), 2.0, device="cuda").half()
+    for call in (lambda: cache.store(0, k, k, [0, 1]), lambda: cache.fork([0, 1], [3, 4])):
+        cache.page_table[0, 1] = page
+        others = cache.page_table[2, :3].long()
+        call()
+        assert int(cache.status) == 8
+        assert bool((cache.pages[0, others] == 1).all())
+        with pytest.raises(tk.TKError, match="outside the pool"):
+            cache.check()
+        with pytest.raises(tk.TKError):
+            tk.check_device_errors(cuda_device)
+        cache.restore(saved)
+    cache.check()

@@ -12,7 +12,10 @@
 // A call applies whole or not at all: its entries are checked before anything
 // is written, a refused call sets a bit of the status word and the device
 // error word, and while the status word is set later calls on the cache
-// change nothing. Entries with slot -1 are padding and are skipped.
+// change nothing. The pages that a table names are not among what is checked
+// first: one outside the pool, which these calls never leave there, is skipped
+// and reported by fork and store when they reach it, with the rest of the call
+// applied or not. Entries with slot -1 are padding and are skipped.
 //
 // These kernels are bound by latency (integer work on a few kB, one CTA that
 // scans the free bits: 7 us for 640 pages of 8 prompts) and, where data moves,
@@ -478,7 +481,7 @@ __global__ void __launch_bounds__(256) store_kernel(Books b, StoreParams p) {
   uint32_t* seen = reinterpret_cast<uint32_t*>(sh);  // [max_seqs / 32]
   for (int i = threadIdx.x; i < (b.max_seqs + 31) / 32; i += blockDim.x) seen[i] = 0u;
   grid_dep_wait();
-  const int status = *b.status;  // only a refusal of this very list can set it meanwhile
+  const int status = *b.status;  // a refusal of this very list, or a page outside the pool, can set it meanwhile
   if (__syncthreads_or(status)) return;
   const int ps = 1 << b.page_shift;
   // every CTA checks every row, so that all agree whether the call applies

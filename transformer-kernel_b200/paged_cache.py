@@ -3,7 +3,7 @@
 ``PagedCache`` keeps the keys and values of many sequences in fixed-size
 pages of one fp16 pool ``[layers, num_pages, 2 (k, v), kv_heads, page_size,
 head_dim]`` and its books (page table, lengths, reference counts) in int32
-tensors on the same device, so a serving loop never waits for the device:
+tensors on the same device, so a serving loop need not wait for the device:
 
     cache = PagedCache(num_layers=4, num_pages=4096, page_size=64, kv_heads=16, head_dim=64,
                        max_seqs=64, max_pages_per_seq=128)
@@ -15,17 +15,25 @@ tensors on the same device, so a serving loop never waits for the device:
 
 ``fork`` lets a sequence continue in several ways (full pages are shared, a
 partial last one is copied), ``release`` frees, ``compact`` moves the pages in
-use to the lowest numbers. Every method is one or two launches on the current
-stream and can be captured into a CUDA graph. Slot lists are int32 tensors on
-the cache's device (slot -1 is padding) or Python ints, each slot at most
-once. A call applies whole or not at all: one that the device refuses (out of
-pages, a slot named twice, a sequence longer than its row) changes nothing and
-sets the status word, after which the cache's calls do nothing -- ``attend``
-leaves its output unwritten -- until ``check()`` has raised the reason and
-``restore`` / ``load`` / ``reset`` has put the books in order. Calls on one
-cache must be ordered on the GPU (one stream, or streams that wait for each
-other). The reference recomputes all keys and values in every forward
-(src/optimized.py:488-554), so nothing here has a counterpart in it.
+use to the lowest numbers. Every call is one or two launches on the current
+stream. Slot lists are int32 tensors on the cache's device (slot -1 is
+padding) or Python ints, each slot at most once (a fork's parents any number
+of times). With tensors nothing waits for the device and a call can be
+captured into a CUDA graph; lists of ints are uploaded by a copy that waits
+for the stream and cannot be captured, and so it is with ``copy_pages``, which
+takes nothing else, ``load`` from host tensors and ``check``.
+
+A call applies whole or not at all: one that the device refuses (out of pages,
+a slot named twice, a sequence longer than its row) changes nothing in the
+cache and sets the status word, after which the cache's calls do nothing --
+``attend`` leaves its output unwritten -- until ``check()`` has raised the
+reason and ``restore`` / ``load`` / ``reset`` has put the books in order. The
+output of an ``attend`` that is itself refused is unspecified. A page table
+that names pages outside the pool (books from elsewhere) and a wait that gives
+up are only found while a call runs: it is reported too, but may have applied
+in part. Calls on one cache must be ordered on the GPU (one stream, or streams
+that wait for each other). The reference recomputes all keys and values in every
+forward (src/optimized.py:488-554), so nothing here has a counterpart in it.
 """
 
 from __future__ import annotations
@@ -176,7 +184,9 @@ class PagedCache:
 
     def fork(self, parents: Slots, children: Slots) -> None:
         """Empty slot ``children[i]`` becomes a copy of ``parents[i]``: full
-        pages are shared, the used rows of a partial last page are copied."""
+        pages are shared, the used rows of a partial last page are copied.
+        Store the parents' reserved tokens first: what is stored in a shared
+        page later is the other holders' as well."""
         p, c = self._ints(parents, "parents"), self._slots(children)
         self._same_length(p, c)
         self._call("tk_cache_fork", p.data_ptr(), c.data_ptr(), p.numel())
