@@ -231,3 +231,14 @@ def test_repeats_bit_for_bit_and_replays(cuda_device):
         second = kernels.window_attention(q, k, v, 0.1, 256, 4, lens)
     torch.cuda.synchronize()
     assert torch.equal(second, first)
+
+
+@gpu
+@pytest.mark.parametrize("hd", [8, 64, 128, 256])
+def test_one_head_with_its_rows_next_to_each_other(cuda_device, hd):
+    """[B, 1, S, hd] contiguous keys and values, and a single query head: a
+    token's row begins where the one before ends."""
+    for B, H, S in ((1, 1, 130), (3, 4, 200), (2, 1, 1)):
+        q, k, v = inputs(B, H, 1, S, hd, seed=S)
+        got = check(q, k, v, 70, 2)
+        assert torch.equal(got, check(q.contiguous(), k.contiguous(), v.contiguous(), 70, 2))

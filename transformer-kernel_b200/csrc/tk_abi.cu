@@ -867,7 +867,7 @@ int map_bhsd(const char* fn, CUtensorMap* map, const void* base, int64_t B, int6
   if (sb <= 0 || sh <= 0 || ss <= 0 || sb % 8 || sh % 8 || ss % 8 || !aligned(base, 16))
     return fail(TK_ERR_INVALID, "%s: q/k/v need 16-byte aligned bases and positive strides (multiples of 8 elements)",
                 fn);
-  const bool inner = sh < ss;
+  const bool inner = H == 1 || sh < ss;
   const int64_t d1 = inner ? H : S, d2 = inner ? S : H, s1 = inner ? sh : ss, s2 = inner ? ss : sh;
   if (s1 < hd || s2 < s1 * d1 || sb < s2)
     return fail(TK_ERR_UNSUPPORTED, "%s: strides (b=%lld, h=%lld, s=%lld) overlap or are not batch-major", fn, (long long)sb, (long long)sh,
