@@ -242,3 +242,35 @@ def test_one_head_with_its_rows_next_to_each_other(cuda_device, hd):
         q, k, v = inputs(B, H, 1, S, hd, seed=S)
         got = check(q, k, v, 70, 2)
         assert torch.equal(got, check(q.contiguous(), k.contiguous(), v.contiguous(), 70, 2))
+
+
+def one_entry_strides():
+    """(k, v, whether their strides agree where they mean something)"""
+    flat = torch.zeros(8192).half()
+    view = lambda shape, strides: torch.as_strided(flat, shape, strides)  # noqa: E731
+    return [(view((1, 2, 8, 64), (8192, 64, 128, 1)), view((1, 2, 8, 64), (3, 64, 128, 1)), True),
+            (view((1, 1, 8, 64), (512, 512, 64, 1)), view((1, 1, 8, 64), (512, 7, 64, 1)), True),
+            (view((2, 2, 1, 64), (128, 64, 128, 1)), view((2, 2, 1, 64), (128, 64, 9, 1)), True),
+            (view((1, 2, 8, 64), (8192, 64, 128, 1)), view((1, 2, 8, 64), (8192, 512, 64, 1)), False)]
+
+
+def test_strides_of_one_entry_are_not_compared():
+    for k, v, same in one_entry_strides():
+        q = torch.zeros(k.shape[0], 4, k.shape[2], 64).half()
+        with pytest.raises(tk.TKError, match="no CPU fallback" if same else "identical strides"):
+            kernels.window_attention(q, k, v, 1.0, 4)
+
+
+@gpu
+def test_strides_of_one_entry_may_differ(cuda_device):
+    """k and v whose strides differ only where a dimension has one entry give
+    what contiguous copies give."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    for k0, v0, same in one_entry_strides():
+        if not same:
+            continue
+        k, v = (torch.as_strided(torch.randn(8192, generator=g, device="cuda").half(), t.shape, t.stride())
+                for t in (k0, v0))
+        q = torch.randn(k.shape[0], 4, k.shape[2], 64, generator=g, device="cuda").half()
+        got = check(q, k, v, 4, 1)
+        assert torch.equal(got, check(q, k.contiguous(), v.contiguous(), 4, 1))

@@ -91,7 +91,8 @@ def window_attention(
 
     ``q`` is ``[B, H, S, hd]``, ``k`` and ``v`` ``[B, Hkv, S, hd]`` with H a
     multiple of Hkv (query head h reads head ``h // (H // Hkv)``), any strides
-    with a contiguous last dimension, shared by k and v. ``kv_len`` (int32
+    with a contiguous last dimension, shared by k and v (in dimensions of more
+    than one entry). ``kv_len`` (int32
     ``[B]``, optional) masks keys ``>= kv_len[b]``; what they hold is never
     used. Rows that see no key are zero. The other values of k and v must be
     finite: inside a tile a masked weight is 0 times the value. Backed by
@@ -108,7 +109,9 @@ def window_attention(
         raise tk.TKError("window_attention", -2, "q/k/v must be float16")
     q_b, q_h, q_s, q_1 = q.stride()
     k_b, k_h, k_s, k_1 = strides = k.stride()
-    if strides != v.stride() or q_1 != 1 or k_1 != 1:
+    # the stride of a dimension of one entry means nothing
+    if q_1 != 1 or k_1 != 1 or (strides != v.stride() and any(
+            n > 1 and a != b for n, a, b in zip(k.shape, strides, v.stride()))):
         raise tk.TKError("window_attention", -1, "k and v need identical strides, and all a contiguous last dimension")
     dev = q.device
     if dev.type != "cuda" or k.device != dev or v.device != dev:
