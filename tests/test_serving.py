@@ -239,3 +239,38 @@ def test_prefill_reads_a_mask_that_is_filled_again(cuda_device):
             model.prefill(x, cache, [0, 1], mask)
     assert cache.seq_lens.tolist() == [24, 5, 7, 24, 1, 2, 24, 24]
     cache.check()
+
+
+@gpu
+def test_calls_refused_on_the_host_leave_the_books(cuda_device):
+    """What a serving call raises for, it raises for before a token is
+    reserved; a window beyond any sequence is none."""
+    model = make_model().cuda()
+    cache = make_cache(model)
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(2, 5, 128, generator=g).cuda()
+    ones = torch.ones(2, 5, dtype=torch.bool, device="cuda")
+    with torch.inference_mode():
+        want = [stack(model, s) for s in x]
+        out = model.prefill(x[:, :4], cache, [0, 1], window=2 ** 40)
+        for b in range(2):
+            agrees(out[b], want[b][:4])
+        books = cache._books.clone()
+        for error, call in (
+            (ValueError, lambda: model.decode_step(x[:, 4], cache, [0, 1], max_len=-1)),
+            (ValueError, lambda: model.decode_step(x[:, 4], cache, [0, 1], window=-1)),
+            (TypeError, lambda: model.decode_step(x[:, 4], cache, [0, 1], window=8.0)),
+            (TypeError, lambda: model.decode_step(x[:, 4], cache, [0, 1], max_len=8.0)),
+            (ValueError, lambda: model.decode_step(x[:, 4], cache, [0, 1, 2])),
+            (TypeError, lambda: model.prefill(x, cache, [2, 3], window=4, sinks=1.5)),
+            (ValueError, lambda: model.prefill(x, cache, [2, 3], ones[:, :4])),
+            (ValueError, lambda: model.prefill(x, cache, [2, 3], ones[:1])),
+            (ValueError, lambda: model.prefill(x, cache, [2, 3, 4], ones)),
+            (tk.TKError, lambda: model.prefill(x, cache, [2, 3], torch.tensor([[1, 0, 1, 0, 0]] * 2).cuda())),
+        ):
+            with pytest.raises(error):
+                call()
+            assert torch.equal(cache._books, books)
+        out = model.decode_step(x[:, 4], cache, [0, 1], window=2 ** 40, sinks=2 ** 33, max_len=2 ** 62)
+        agrees(out, torch.stack([w[4] for w in want]))
+    cache.check()

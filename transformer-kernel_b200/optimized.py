@@ -38,6 +38,7 @@ new token (:488-554).
 
 from __future__ import annotations
 
+import operator
 import weakref
 from dataclasses import dataclass, replace
 from typing import List, Optional
@@ -454,7 +455,9 @@ class OptimizedTransformer(nn.Module):
             return self._body(B, S, lengths, bufs, weights, out)
 
     # -- serving ------------------------------------------------------------------
-    def _check_cache(self, cache: PagedCache, device: torch.device, window: int, sinks: int) -> None:
+    def _check_cache(self, cache: PagedCache, device: torch.device, *sizes: int) -> tuple:
+        """What a serving call can refuse on the host, before the cache's books
+        change. Returns ``sizes`` (window, sinks, ...) as the kernels take them."""
         if not self.config.causal:
             raise tk.TKError("serving", -2, "only a causal model can keep its keys and values while it generates")
         want = (len(self.layers), self.num_heads, self.head_dim)
@@ -463,8 +466,10 @@ class OptimizedTransformer(nn.Module):
                              f"{(cache.num_layers, cache.kv_heads, cache.head_dim)}")
         if cache.device != device:
             raise tk.TKError("device", -1, f"tensors on different devices: {device} vs {cache.device}")
-        if window < 0 or sinks < 0:
-            raise ValueError("window and sinks cannot be negative")
+        sizes = tuple(operator.index(n) for n in sizes)
+        if any(n < 0 for n in sizes):
+            raise ValueError("window, sinks and max_len cannot be negative")
+        return tuple(min(n, 2 ** 31 - 1) for n in sizes)  # no sequence is that long
 
     @_outside_compile
     def prefill(
@@ -483,18 +488,23 @@ class OptimizedTransformer(nn.Module):
         this call, which waits for the device; with one, ``prefill`` cannot be
         captured into a CUDA graph."""
         self._check_input(x)
-        self._check_cache(cache, x.device, window, sinks)
+        window, sinks = self._check_cache(cache, x.device, window, sinks)
         B, S, d = x.shape
         if B * S == 0:
             raise ValueError(f"prompts need at least one row and one token, got {tuple(x.shape)}")
         lengths = None
         if valid_token_mask is not None and not self.settings.assume_dense_mask:
+            if valid_token_mask.shape != (B, S):
+                raise ValueError(f"expected a mask of shape {(B, S)}, got {tuple(valid_token_mask.shape)}")
             if torch.cuda.is_current_stream_capturing():
                 raise tk.TKError("prefill", -2, "the lengths of a mask cannot be read while a CUDA graph is captured")
             # the lengths go into the cache's books: never those of an earlier call
             lengths, _ = self._count_prefixes(valid_token_mask)
         counts = torch.full((B,), S, dtype=torch.int32, device=x.device) if lengths is None else lengths
         slots = cache._slots(slots)
+        weights = self._weights()
+        with torch.cuda.device(x.device):
+            bufs = self._activations(B, S, d, weights[0].ffn_in_w.shape[0], x.device)
         cache.reserve(slots, counts, require_empty=True)
 
         def attend(layer, q, k, v, ctx):
@@ -505,9 +515,7 @@ class OptimizedTransformer(nn.Module):
             else:
                 self._launch("attn", kernels.flash_attention, q, k, v, self.attn_scale, True, kv_len=lengths, out=ctx)
 
-        weights = self._weights()
         with torch.cuda.device(x.device):
-            bufs = self._activations(B, S, d, weights[0].ffn_in_w.shape[0], x.device)
             self._head(x, bufs, weights)
             return self._finish(x, self._body(B, S, lengths, bufs, weights, attend=attend))
 
@@ -529,11 +537,14 @@ class OptimizedTransformer(nn.Module):
         if x.dim() != 2 or x.shape[1] != self.d_model:
             raise ValueError(f"expected x of shape [B, {self.d_model}], got {tuple(x.shape)}")
         self._check_input(x[:, None])
-        self._check_cache(cache, x.device, window, sinks)
+        window, sinks, max_len = self._check_cache(cache, x.device, window, sinks, max_len)
         B, d = x.shape
         if B == 0:
             return x.clone()
         slots = cache._slots(slots)
+        weights = self._weights()
+        with torch.cuda.device(x.device):
+            bufs = self._activations(B, 1, d, weights[0].ffn_in_w.shape[0], x.device)
         cache.reserve(slots, torch.ones(B, dtype=torch.int32, device=x.device))
 
         def attend(layer, q, k, v, ctx):
@@ -541,9 +552,7 @@ class OptimizedTransformer(nn.Module):
                          v_new=v[:, :, 0], slots=slots, window=window, sinks=sinks, max_len=max_len,
                          out=ctx.view(B, d))
 
-        weights = self._weights()
         with torch.cuda.device(x.device):
-            bufs = self._activations(B, 1, d, weights[0].ffn_in_w.shape[0], x.device)
             self._head(x[:, None], bufs, weights)
             return self._finish(x, self._body(B, 1, None, bufs, weights, attend=attend).view(B, d))
 
