@@ -113,3 +113,31 @@ def test_resid_ln_workspace_and_support_on_host():
                                 16, 4096, None) == -2
     assert lib.tk_gemm_resid_ln(16, 64, 16, 64, 16, 16, 1024, 16, 1024, 16, 16, 1e-5, 16, 1, 1024, None, 0, 8, 1024,
                                 64, None, 0, None) == -1
+
+
+def test_stream_handle_without_the_raw_lookup(monkeypatch):
+    """A torch without the private lookup still gives the current stream."""
+    import types
+
+    import torch
+
+    asked = []
+    monkeypatch.setattr(tk, "_raw_stream", None)
+    monkeypatch.setattr(torch.cuda, "current_stream",
+                        lambda device: asked.append(device) or types.SimpleNamespace(cuda_stream=1234))
+    assert tk.stream_handle(torch.device("cuda", 1)) == 1234 and asked == [torch.device("cuda", 1)]
+
+
+@pytest.mark.gpu
+def test_stream_handle_is_the_current_stream(cuda_device, monkeypatch):
+    import torch
+
+    def handles():
+        with torch.cuda.stream(side):
+            return [tk.stream_handle(d) for d in (cuda_device, torch.device("cuda"))]
+
+    side = torch.cuda.Stream()
+    assert handles() == [side.cuda_stream] * 2
+    assert tk.stream_handle(cuda_device) == torch.cuda.current_stream().cuda_stream != side.cuda_stream
+    monkeypatch.setattr(tk, "_raw_stream", None)
+    assert handles() == [side.cuda_stream] * 2

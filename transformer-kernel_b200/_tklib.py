@@ -135,11 +135,17 @@ def dtype_code(dt: torch.dtype) -> int:
     raise TKError("dtype", -1, f"unsupported dtype {dt}; the kernels take float32 or float16")
 
 
+# The raw handle without the torch.cuda.Stream object around it, which costs
+# 2 us a call; not part of torch's public interface, so it may be missing.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device) -> int:
-    """cudaStream_t of the device's current stream (the raw handle, without
-    the torch.cuda.Stream object around it, which costs 2 us a call)."""
+    """cudaStream_t of the device's current stream."""
+    if _raw_stream is None:
+        return torch.cuda.current_stream(device).cuda_stream
     index = device.index
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+    return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
 def call_on(device: torch.device, name: str, *args) -> int:
