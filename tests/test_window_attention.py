@@ -274,3 +274,10 @@ def test_strides_of_one_entry_may_differ(cuda_device):
         q = torch.randn(k.shape[0], 4, k.shape[2], 64, generator=g, device="cuda").half()
         got = check(q, k, v, 4, 1)
         assert torch.equal(got, check(q, k.contiguous(), v.contiguous(), 4, 1))
+
+
+@gpu
+@pytest.mark.parametrize("window, sinks", [(2 ** 63 - 1, 0), (2 ** 63 - 1, 2 ** 63 - 1), (1, 2 ** 63 - 1), (2 ** 31, 2 ** 31)])
+def test_windows_and_first_tokens_beyond_any_length(cuda_device, window, sinks):
+    q, k, v = inputs(2, 2, 1, 300, 64)
+    assert torch.equal(check(q, k, v, window, sinks), check(q, k, v, 300, 0))

@@ -970,7 +970,8 @@ int tk_attn_window(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_
   p.kv_len = kv_len;
   p.hd = static_cast<int>(hd);
   p.wait_limit_ns = g_wait_limit_ns.load();
-  const bool small = static_cast<double>(B) * H * S * std::min(window + sinks, S) * hd <= kSmallAttnWork;
+  const int64_t seen = std::min<int64_t>(static_cast<int64_t>(p.window) + p.sinks, S);
+  const bool small = static_cast<double>(B) * H * S * seen * hd <= kSmallAttnWork;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (hd == 256) return launch_window<256>(info, 4, maps, p, small, s);
   if (hd == 128) return launch_window<128>(info, 3, maps, p, small, s);
