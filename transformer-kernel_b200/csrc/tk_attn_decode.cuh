@@ -24,9 +24,9 @@
 // keep their accumulators, the running maximum and the sum in registers in
 // fp32; P is rounded to fp16 for the second product (half a step, 2^-11
 // relative, as in the prompt kernel). No barrier joins the warps until their
-// results are merged. Measured: 4 x 100,000 keys, 16 heads of 64: 252 us (6.5
-// TB/s, the copy's rate); 64 sequences, 32 / 8 heads of 128, window 2000: 76 us
-// (6.1 TB/s); one sequence of 97 tokens: 3.2 us in a graph.
+// results are merged. Measured: 4 x 100,000 keys, 16 heads of 64: 264 us (6.2
+// TB/s, 0.95 of the copy's rate); 64 sequences, 32 / 8 heads of 128, window
+// 2000: 79 us (5.9 TB/s); one sequence of 97 tokens: 3.1 us in a graph.
 #pragma once
 
 #include <cuda.h>
@@ -60,11 +60,12 @@ struct Tiles {
 
 // A step's latency (barrier, products, two shuffles, exponentials: 0.5 us at
 // 16 keys, 0.7 at 32, 0.9 at 64, hd 64) is what a lone warp is bound by, so
-// steps are as large as leaves the rings of 12 warps an SM (hd 128: 4 warps)
-// about 200 KB in flight. 32 keys against 16: 8 x 16,384 keys, 16 heads of 64,
-// one CTA each, 98 us against 150; 8 x 1024, 8 groups of hd 128, 11.7 against
-// 16.2; 64 keys lose where CTAs are many (256 short sequences, 48 us against
-// 29).
+// steps are as large as leaves the rings room for several warps an SM: 12 with
+// 192 KB in flight at hd 64, 4 with 128 KB at hd 128 and 192 KB at hd 256, 16
+// with 64 and 128 KB at hd 16 and 32. 32 keys against 16: 8 x 16,384 keys, 16
+// heads of 64, one CTA each, 98 us against 150; 8 x 1024, 8 groups of hd 128,
+// 11.7 against 16.2; 64 keys lose where CTAs are many (256 short sequences, 48
+// us against 29).
 template <int HD>
 struct Cfg : Tiles<HD, HD == 256 ? 16 : 32, HD == 256 ? 3 : 2> {
   using Base = Tiles<HD, HD == 256 ? 16 : 32, HD == 256 ? 3 : 2>;

@@ -27,11 +27,14 @@
 //  - hd 128: the score and output tiles of two groups fill TMEM, so P_g
 //    overwrites the first half of S_g, and S_g of the next step is issued once
 //    P_g's product is complete; hd 256: one query tile per item.
-// Bound by the softmax warps' latency (hd <= 64; no pipe above 52%: a quarter
-// of the exponentials on the FMA pipe, none cost +2%, half +12%) and by the
-// chain scores -> softmax -> product of a group (hd 128). Measured: one prompt
-// of 100,000 tokens, 16 heads of 64, window 4096: 2.20 ms (760 TFLOP/s of
-// visible pairs); 4 x 8191, 32 / 8 heads of 128, window 1024: 0.62 ms (840).
+// Bound by the softmax warps' latency (hd <= 64: the SFU, the busiest pipe, is
+// at 56%, the tensor pipe at 37%; a quarter of the exponentials go on the FMA
+// pipe, none cost +2%, half +12%) and by the chain scores -> softmax -> product
+// of a group (hd 128: tensor pipe 48%, SFU 37%). Measured under steady load, in
+// brackets ten calls after a pause, before the clock falls: one prompt of
+// 100,000 tokens, 16 heads of 64, window 4096: 2.48 ms, 673 TFLOP/s of visible
+// pairs (2.21, 755); 4 x 8191, 32 / 8 heads of 128, window 1024: 0.74 ms, 707
+// (0.64, 815); 4 x 8191, 16 / 4 heads of 256, window 1024: 0.83 ms, 630 (0.76).
 //
 // Value rows at and past kv_len are zeroed in shared memory before the product
 // reads them: their P is 0, but 0 times what they hold may not be (keys need

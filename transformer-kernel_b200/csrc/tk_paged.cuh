@@ -20,7 +20,8 @@
 // These kernels are bound by latency (integer work on a few kB, one CTA that
 // scans the free bits: 7 us for 640 pages of 8 prompts) and, where data moves,
 // by HBM, 2 bytes of traffic per byte: store of 45,000 tokens x 16 heads of 64
-// in 64 us (5.8 TB/s), a compaction that moves 0.37 GB in 127 us (5.8).
+// in 64 us (5.8 TB/s), a compaction that moves 0.37 GB in 127 us (5.8), 1000
+// pages of 0.5 MB copied in 177 us (5.9).
 #pragma once
 
 #include <cuda_fp16.h>

@@ -532,8 +532,9 @@ class OptimizedTransformer(nn.Module):
         """One more token for each sequence: ``x`` ``[B, d]`` is appended to
         ``slots`` and attends over what the cache holds. Returns ``[B, d]`` in
         x's dtype; rows with slot -1 are padding and hold nothing of use. Can
-        be captured into a CUDA graph (with ``slots`` a tensor). ``max_len``:
-        as for ``PagedCache.attend``."""
+        be captured into a CUDA graph (with ``slots`` a tensor), which serves
+        until the weights are loaded again. ``max_len``: as for
+        ``PagedCache.attend``."""
         if x.dim() != 2 or x.shape[1] != self.d_model:
             raise ValueError(f"expected x of shape [B, {self.d_model}], got {tuple(x.shape)}")
         self._check_input(x[:, None])

@@ -265,10 +265,12 @@ class PagedCache:
         ``q`` is ``[B, H, head_dim]`` fp16 (any strides, contiguous last
         dimension); query head h reads key-value head ``h // (H // kv_heads)``.
         With ``k_new`` / ``v_new`` ``[B, kv_heads, head_dim]`` the token's key
-        and value are written into the cache as well. ``window`` > 0 hides the
+        and value are written into the cache as well, for all rows or none. ``window`` > 0 hides the
         keys that lie ``window`` or more tokens back, except the first
         ``sinks``. Without ``slots`` row b is sequence b; rows with slot -1
-        are left as they are, an empty sequence gives zeros."""
+        are left as they are, an empty sequence gives zeros. ``max_len`` > 0
+        bounds the rows' lengths where the caller knows better than the
+        table's width; it only helps to choose how the work is divided."""
         K, hd = self.kv_heads, self.head_dim
         shape = q.shape
         if len(shape) != 3 or shape[2] != hd or shape[1] == 0 or shape[1] % K:
