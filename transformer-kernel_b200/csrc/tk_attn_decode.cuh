@@ -91,7 +91,7 @@ struct Params {
   int hd;                 // head_dim of the data: HD, or 8 in the HD = 16 kernel (zero-padded by TMA)
   int window, sinks;      // window 0: every key
   float scale_log2;
-  uint64_t wait_limit_ns;
+  uint64_t wait_limit_ns; // 0: every wait for keys gives up at once
   int store_ctas;         // first CTAs of decode_kernel: they store the new tokens (none without k_new)
   // split over the grid (decode_split_kernel)
   int ctas, min_steps;    // CTAs of the grid; fewest steps one takes
